@@ -13,6 +13,11 @@ from .flash_attention_interface import (  # noqa: F401
     flash_attn_varlen_qkvpacked_func,
     flash_attn_with_kvcache,
 )
+from .diff_attention_interface import (  # noqa: F401
+    flash_diff_attn_func,
+    flash_diff_attn_varlen_func,
+    flash_diff_attn_with_kvcache,
+)
 
 
 
@@ -54,4 +59,7 @@ __all__ = [
     "flash_attn_varlen_kvpacked_func",
     "flash_attn_varlen_qkvpacked_func",
     "flash_attn_with_kvcache",
+    "flash_diff_attn_func",
+    "flash_diff_attn_varlen_func",
+    "flash_diff_attn_with_kvcache",
 ]

@@ -28,7 +28,8 @@ LIB_PATH = PKG_DIR / "libfa_b200.so"
 EXT_NAME = "_fa_b200_torch"
 EXT_PATH = PKG_DIR / f"{EXT_NAME}.so"
 
-CUDA_SOURCES = ["common.cu", "fwd_sm100.cu", "bwd_sm100.cu", "bwd_fused_sm100.cu", "kvcache_sm100.cu", "combine.cu"]
+CUDA_SOURCES = ["common.cu", "fwd_sm100.cu", "bwd_sm100.cu", "bwd_fused_sm100.cu", "kvcache_sm100.cu", "combine.cu",
+                "diff.cu"]
 # Ahead of the compiler's own -lstdc++, which is an archive in some installations: a second C++ runtime in the extension takes the
 # place of a part of the one torch uses, and formatting a number for an exception then crashes the process.
 CXX_RUNTIME = "-l:libstdc++.so.6"

@@ -28,6 +28,12 @@ EXPORTED_SYMBOLS = (
     "fa_combine",
     "fa_combine_gather",
     "fa_sum_gather",
+    "fa_diff_fwd_workspace_bytes",
+    "fa_diff_fwd",
+    "fa_diff_bwd_workspace_bytes",
+    "fa_diff_bwd",
+    "fa_diff_kvcache_workspace_bytes",
+    "fa_diff_kvcache",
 )
 
 _i64, _i32, _f32, _vp, _sz = C.c_int64, C.c_int32, C.c_float, C.c_void_p, C.c_size_t
@@ -79,6 +85,22 @@ class FaKvcacheParams(C.Structure):
            ("block_table_batch_stride", _i64), ("max_blocks_per_seq", _i32), ("num_splits", _i32),
            ("workspace", _vp), ("workspace_bytes", _sz)]
     )
+
+
+class FaDiffWeights(C.Structure):
+    _fields_ = [("lam", _vp), ("stride", _i64), ("count", _i32), ("is_half", _i32)]
+
+
+class FaDiffFwdParams(C.Structure):
+    _fields_ = [("base", FaFwdParams), ("weights", FaDiffWeights), ("o2", _vp), *_strides("o2"), ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class FaDiffBwdParams(C.Structure):
+    _fields_ = [("base", FaBwdParams), ("weights", FaDiffWeights), ("o2", _vp), *_strides("o2"), ("dlam", _vp)]
+
+
+class FaDiffKvcacheParams(C.Structure):
+    _fields_ = [("base", FaKvcacheParams), ("weights", FaDiffWeights)]
 
 
 class FaCombineParams(C.Structure):
@@ -139,6 +161,11 @@ def lib() -> C.CDLL:
         l.fa_bwd_workspace_bytes.argtypes = [C.POINTER(FaBwdParams)]
         l.fa_kvcache_workspace_bytes.restype = _sz
         l.fa_kvcache_workspace_bytes.argtypes = [C.POINTER(FaKvcacheParams)]
+        for name, struct in (("fa_diff_fwd", FaDiffFwdParams), ("fa_diff_bwd", FaDiffBwdParams), ("fa_diff_kvcache", FaDiffKvcacheParams)):
+            fn, size = getattr(l, name), getattr(l, name + "_workspace_bytes")
+            fn.restype, size.restype = C.c_int, _sz
+            fn.argtypes = [C.POINTER(struct), _vp, _i32, _vp] if name == "fa_diff_kvcache" else [C.POINTER(struct), _vp]
+            size.argtypes = [C.POINTER(struct)]
         l.fa_kvcache_num_splits.restype = C.c_int
         l.fa_kvcache_num_splits.argtypes = [C.POINTER(FaKvcacheParams)]
         _lib = l

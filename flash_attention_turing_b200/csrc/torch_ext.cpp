@@ -53,13 +53,82 @@ void check_lse_view(const at::Tensor& l, int64_t b, int64_t h, int64_t rows, con
               " must have unit stride along the rows and batches h row pitches apart");
 }
 
+// ---- differential attention: what a call has besides q, k and v ----
+struct Differential {
+  at::Tensor lam;
+  bool keep = false;  // forward: o2 is wanted, for the backward
+  at::Tensor o2;      // A_2 V
+  at::Tensor dlam;
+};
+
+FaDiffWeights diff_weights(const at::Tensor& lam, const at::Tensor& q, int64_t num_heads) {
+  TORCH_CHECK(lam.is_cuda() && lam.device() == q.device(), "lam must be a CUDA tensor on the device of q");
+  TORCH_CHECK(lam.scalar_type() == at::kFloat || lam.scalar_type() == at::kHalf, "lam must be a float32 or float16 tensor");
+  TORCH_CHECK(lam.dim() <= 1 && (lam.numel() == 1 || lam.numel() == num_heads), "lam must have one element or shape [nheads_q]");
+  FaDiffWeights w = {};
+  w.lam = lam.data_ptr();
+  w.count = static_cast<int32_t>(lam.numel());
+  w.stride = lam.dim() == 1 ? lam.stride(0) : 0;
+  w.is_half = lam.scalar_type() == at::kHalf;
+  return w;
+}
+
+void check_same_device(const at::Tensor& q, std::initializer_list<at::Tensor> others) {
+  for (const at::Tensor& t : others) TORCH_CHECK(t.device() == q.device(), "all tensors must be on the device of q");
+}
+
+// Scratch memory of a call; 256-byte aligned, as the caching allocator gives it
+at::Tensor scratch(size_t bytes, const at::Tensor& like) {
+  return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(torch::kUInt8));
+}
+
+int launch_forward(const FaFwdParams& p, Differential* diff, const at::Tensor& q, int64_t num_heads) {
+  if (diff == nullptr) return fa_fwd(&p, current_stream());
+  FaDiffFwdParams d = {};
+  d.base = p;
+  d.weights = diff_weights(diff->lam, q, num_heads);
+  if (diff->keep) {
+    const at::Tensor& o2 = diff->o2;
+    const int64_t batch = o2.dim() == 4 ? 1 : 0;  // packed tensors have no batch dimension
+    d.o2 = o2.data_ptr();
+    d.o2_batch_stride = batch ? o2.stride(0) : 0, d.o2_row_stride = o2.stride(batch), d.o2_head_stride = o2.stride(batch + 1);
+  }
+  at::Tensor workspace = scratch(fa_diff_fwd_workspace_bytes(&d), q);
+  d.workspace = workspace.data_ptr();
+  d.workspace_bytes = workspace.numel();
+  return fa_diff_fwd(&d, current_stream());
+}
+
+// p: everything but the workspace
+void launch_backward(FaBwdParams& p, Differential* diff, const at::Tensor& q, int64_t num_heads) {
+  if (diff == nullptr) {
+    at::Tensor workspace = scratch(fa_bwd_workspace_bytes(&p), q);
+    p.workspace = workspace.data_ptr();
+    p.workspace_bytes = workspace.numel();
+    check_rc(fa_bwd(&p, current_stream()), "fa_bwd");
+    return;
+  }
+  FaDiffBwdParams d = {};
+  d.base = p;
+  d.weights = diff_weights(diff->lam, q, num_heads);
+  const at::Tensor& o2 = diff->o2;
+  const int64_t batch = o2.dim() == 4 ? 1 : 0;
+  d.o2 = o2.data_ptr();
+  d.o2_batch_stride = batch ? o2.stride(0) : 0, d.o2_row_stride = o2.stride(batch), d.o2_head_stride = o2.stride(batch + 1);
+  d.dlam = diff->dlam.data_ptr();
+  at::Tensor workspace = scratch(fa_diff_bwd_workspace_bytes(&d), q);
+  d.base.workspace = workspace.data_ptr();
+  d.base.workspace_bytes = workspace.numel();
+  check_rc(fa_diff_bwd(&d, current_stream()), "fa_diff_bwd");
+}
+
 // ---- dense forward (mha_fwd, flash_api.cpp:188-256) ----
 // out_, lse_ (optional, after the reference's five arguments): write O and LSE there instead of into new tensors
 // (strided views are fine: e.g. a block of rows of a larger buffer).  causal_shift_ (optional): with is_causal,
 // key j is visible to query i iff j <= i + causal_shift instead of the bottom-right alignment.
-std::vector<at::Tensor> mha_fwd(at::Tensor q, at::Tensor k, at::Tensor v, const double softmax_scale,
-                                bool is_causal, c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse_,
-                                c10::optional<int64_t> causal_shift_) {
+std::vector<at::Tensor> dense_forward(at::Tensor q, at::Tensor k, at::Tensor v, const double softmax_scale,
+                                      bool is_causal, c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse_,
+                                      c10::optional<int64_t> causal_shift_, Differential* diff) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k, v must be rank-4 tensors");
   check_half_cuda(q, "q");
   check_half_cuda(k, "k");
@@ -72,20 +141,27 @@ std::vector<at::Tensor> mha_fwd(at::Tensor q, at::Tensor k, at::Tensor v, const 
   TORCH_CHECK(k.size(3) == head_size && v.size(3) == head_size, "q/k/v head_dim must match");
   TORCH_CHECK(num_heads % num_heads_k == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(head_size);
+  const int64_t lse_heads = diff ? 2 * num_heads : num_heads;
+  if (diff) {
+    check_same_device(q, {k, v});
+    diff_weights(diff->lam, q, num_heads);
+  }
   c10::cuda::CUDAGuard guard(q.device());
 
   at::Tensor o = (out_.has_value() && out_->defined()) ? *out_ : torch::empty(q.sizes(), q.options());
   at::Tensor l = (lse_.has_value() && lse_->defined())
-                     ? *lse_ : torch::empty({batch_size, num_heads, seqlen_q}, q.options().dtype(torch::kFloat32));
+                     ? *lse_ : torch::empty({batch_size, lse_heads, seqlen_q}, q.options().dtype(torch::kFloat32));
+  if (diff && diff->keep) diff->o2 = torch::empty(q.sizes(), q.options());
   if (out_.has_value() && out_->defined()) {
     check_half_cuda(o, "out");
     TORCH_CHECK(o.sizes() == q.sizes() && o.device() == q.device(), "out must have the shape and device of q");
   }
-  if (lse_.has_value() && lse_->defined()) check_lse_view(l, batch_size, num_heads, seqlen_q, "lse");
+  if (lse_.has_value() && lse_->defined()) check_lse_view(l, batch_size, lse_heads, seqlen_q, "lse");
   if (batch_size == 0 || seqlen_q == 0) return {o, l};
   if (seqlen_k == 0) {
     o.zero_();
     l.zero_();
+    if (diff && diff->keep) diff->o2.zero_();
     return {o, l};
   }
 
@@ -106,8 +182,14 @@ std::vector<at::Tensor> mha_fwd(at::Tensor q, at::Tensor k, at::Tensor v, const 
     p.is_causal = FA_CAUSAL_SHIFT;
     p.causal_shift = static_cast<int32_t>(*causal_shift_);
   }
-  check_rc(fa_fwd(&p, current_stream()), "fa_fwd");
+  check_rc(launch_forward(p, diff, q, num_heads), diff ? "fa_diff_fwd" : "fa_fwd");
   return {o, l};
+}
+
+std::vector<at::Tensor> mha_fwd(at::Tensor q, at::Tensor k, at::Tensor v, const double softmax_scale,
+                                bool is_causal, c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse_,
+                                c10::optional<int64_t> causal_shift_) {
+  return dense_forward(q, k, v, softmax_scale, is_causal, out_, lse_, causal_shift_, nullptr);
 }
 
 void check_cu_seqlens(const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k) {
@@ -137,19 +219,26 @@ void check_varlen_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor
 }
 
 // ---- varlen forward (mha_varlen_fwd, flash_api.cpp:353-416) ----
-std::vector<at::Tensor> mha_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu_seqlens_q,
+std::vector<at::Tensor> varlen_forward(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu_seqlens_q,
                                        at::Tensor cu_seqlens_k, const int64_t max_seqlen_q,
                                        const int64_t max_seqlen_k, const double softmax_scale,
-                                       bool is_causal) {
+                                       bool is_causal, Differential* diff) {
   check_varlen_qkv(q, k, v);
   check_cu_seqlens(cu_seqlens_q, cu_seqlens_k);
   const int64_t batch_size = cu_seqlens_q.numel() - 1;
   const int64_t num_heads = q.size(1), num_heads_k = k.size(1), head_size = q.size(2);
+  const int64_t lse_heads = diff ? 2 * num_heads : num_heads;
+  if (diff) {
+    check_same_device(q, {k, v, cu_seqlens_q, cu_seqlens_k});
+    diff_weights(diff->lam, q, num_heads);
+  }
   c10::cuda::CUDAGuard guard(q.device());
 
   at::Tensor out = torch::empty_like(q);
-  at::Tensor l = torch::empty({batch_size, num_heads, max_seqlen_q}, q.options().dtype(torch::kFloat32));
-  if (q.size(0) == 0 || k.size(0) == 0 || max_seqlen_q <= 0) return {out.zero_(), l.zero_()};
+  at::Tensor l = torch::empty({batch_size, lse_heads, max_seqlen_q}, q.options().dtype(torch::kFloat32));
+  const bool empty = q.size(0) == 0 || k.size(0) == 0 || max_seqlen_q <= 0;
+  if (diff && diff->keep) diff->o2 = empty ? torch::zeros_like(q) : torch::empty_like(q);
+  if (empty) return {out.zero_(), l.zero_()};
 
   FaFwdParams p = {};
   p.flags = FA_FWD_ZERO_UNUSED_ROWS;  // rows outside every sequence are zero, as in the reference, in O and in the LSE
@@ -167,8 +256,15 @@ std::vector<at::Tensor> mha_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v,
   p.is_causal = is_causal;
   p.cu_seqlens_q = cu_seqlens_q.data_ptr<int>();
   p.cu_seqlens_k = cu_seqlens_k.data_ptr<int>();
-  check_rc(fa_fwd(&p, current_stream()), "fa_fwd");
+  check_rc(launch_forward(p, diff, q, num_heads), diff ? "fa_diff_fwd" : "fa_fwd");
   return {out, l};
+}
+
+std::vector<at::Tensor> mha_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu_seqlens_q,
+                                       at::Tensor cu_seqlens_k, const int64_t max_seqlen_q,
+                                       const int64_t max_seqlen_k, const double softmax_scale,
+                                       bool is_causal) {
+  return varlen_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, nullptr);
 }
 
 // ---- dense backward (mha_bwd, flash_api.cpp:258-351) ----
@@ -189,10 +285,10 @@ at::Tensor grad_destination(const c10::optional<at::Tensor>& given, const at::Te
 
 // dq_, dk_, dv_ (optional, after the reference's eight arguments): write the gradients there instead of
 // into new tensors; strided views are fine (16-byte aligned, strides multiples of 8 elements).
-std::vector<at::Tensor> mha_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
-                                at::Tensor dout, const double softmax_scale, bool is_causal,
-                                c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
-                                c10::optional<at::Tensor> dv_, c10::optional<int64_t> causal_shift_) {
+std::vector<at::Tensor> dense_backward(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
+                                       at::Tensor dout, const double softmax_scale, bool is_causal,
+                                       c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
+                                       c10::optional<at::Tensor> dv_, c10::optional<int64_t> causal_shift_, Differential* diff) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k, v must be rank-4 tensors");
   TORCH_CHECK(out.dim() == 4 && dout.dim() == 4, "out and dout must be rank-4 tensors");
   check_half_cuda(q, "q"); check_half_cuda(k, "k"); check_half_cuda(v, "v");
@@ -206,14 +302,22 @@ std::vector<at::Tensor> mha_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Te
   TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(), "out and dout must match q shape");
   TORCH_CHECK(num_heads % num_heads_k == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(head_size);
-  check_lse_view(l, batch_size, num_heads, seqlen_q, "l");
+  check_lse_view(l, batch_size, diff ? 2 * num_heads : num_heads, seqlen_q, "l");
+  if (diff) {
+    check_same_device(q, {k, v, out, dout, l});
+    diff_weights(diff->lam, q, num_heads);
+    check_half_cuda(diff->o2, "o2");
+    TORCH_CHECK(diff->o2.sizes() == q.sizes() && diff->o2.device() == q.device(), "o2 must have the shape and device of q");
+  }
   c10::cuda::CUDAGuard guard(q.device());
 
   at::Tensor dq = grad_destination(dq_, q, "dq", false);
   at::Tensor dk = grad_destination(dk_, k, "dk", false);
   at::Tensor dv = grad_destination(dv_, v, "dv", false);
+  if (diff) diff->dlam = torch::empty_like(diff->lam, diff->lam.options(), at::MemoryFormat::Contiguous);
   if (batch_size == 0 || seqlen_q == 0 || seqlen_k == 0) {
     dq.zero_(); dk.zero_(); dv.zero_();
+    if (diff) diff->dlam.zero_();
     return {dq, dk, dv};
   }
 
@@ -238,22 +342,25 @@ std::vector<at::Tensor> mha_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Te
     p.is_causal = FA_CAUSAL_SHIFT;
     p.causal_shift = static_cast<int32_t>(*causal_shift_);
   }
-  p.flags = g_bwd_flags;
-  const size_t ws = fa_bwd_workspace_bytes(&p);
-  at::Tensor workspace = torch::empty({static_cast<int64_t>(ws)}, q.options().dtype(torch::kUInt8));
-  p.workspace = workspace.data_ptr();
-  p.workspace_bytes = ws;
-  check_rc(fa_bwd(&p, current_stream()), "fa_bwd");
+  if (!diff) p.flags = g_bwd_flags;
+  launch_backward(p, diff, q, num_heads);
   return {dq, dk, dv};
 }
 
+std::vector<at::Tensor> mha_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
+                                at::Tensor dout, const double softmax_scale, bool is_causal,
+                                c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
+                                c10::optional<at::Tensor> dv_, c10::optional<int64_t> causal_shift_) {
+  return dense_backward(q, k, v, out, l, dout, softmax_scale, is_causal, dq_, dk_, dv_, causal_shift_, nullptr);
+}
+
 // ---- varlen backward (mha_varlen_bwd, flash_api.cpp:418-506) ----
-std::vector<at::Tensor> mha_varlen_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
-                                       at::Tensor dout, at::Tensor cu_seqlens_q, at::Tensor cu_seqlens_k,
-                                       const int64_t max_seqlen_q, const int64_t max_seqlen_k,
-                                       const double softmax_scale, bool is_causal,
-                                       c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
-                                       c10::optional<at::Tensor> dv_) {
+std::vector<at::Tensor> varlen_backward(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
+                                        at::Tensor dout, at::Tensor cu_seqlens_q, at::Tensor cu_seqlens_k,
+                                        const int64_t max_seqlen_q, const int64_t max_seqlen_k,
+                                        const double softmax_scale, bool is_causal,
+                                        c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
+                                        c10::optional<at::Tensor> dv_, Differential* diff) {
   check_varlen_qkv(q, k, v);
   check_cu_seqlens(cu_seqlens_q, cu_seqlens_k);
   check_half_cuda(out, "out");
@@ -263,20 +370,30 @@ std::vector<at::Tensor> mha_varlen_bwd(at::Tensor q, at::Tensor k, at::Tensor v,
   TORCH_CHECK(l.dim() == 3, "l must be rank-3 for varlen_bwd");
   const int64_t batch_size = cu_seqlens_q.numel() - 1;
   const int64_t num_heads = q.size(1), num_heads_k = k.size(1), head_size = q.size(2);
-  TORCH_CHECK(l.size(0) == batch_size && l.size(1) == num_heads && l.size(2) == max_seqlen_q,
+  TORCH_CHECK(l.size(0) == batch_size && l.size(1) == (diff ? 2 * num_heads : num_heads) && l.size(2) == max_seqlen_q,
               "l must have shape [batch_size, nheads_q, max_seqlen_q]");
   TORCH_CHECK(l.is_cuda() && l.scalar_type() == torch::kFloat32 && l.is_contiguous(),
               "l must be a contiguous float32 CUDA tensor");
+  if (diff) {
+    check_same_device(q, {k, v, out, dout, l, cu_seqlens_q, cu_seqlens_k});
+    diff_weights(diff->lam, q, num_heads);
+    check_half_cuda(diff->o2, "o2");
+    TORCH_CHECK(diff->o2.sizes() == q.sizes() && diff->o2.device() == q.device(), "o2 must have the shape and device of q");
+  }
   c10::cuda::CUDAGuard guard(q.device());
 
   // rows outside every sequence are zero, as in the reference (torch::zeros_like, :462-464); the default path clears
   // them itself, a whole pass over the gradients less
   const bool empty = q.size(0) == 0 || k.size(0) == 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0;
-  const int bwd_flags = g_bwd_flags;
+  const int bwd_flags = diff ? 0 : g_bwd_flags.load();
   const bool zero_all = empty || (bwd_flags & FA_BWD_SINGLE_KERNEL) != 0;
   at::Tensor dq = grad_destination(dq_, q, "dq", zero_all);
   at::Tensor dk = grad_destination(dk_, k, "dk", zero_all);
   at::Tensor dv = grad_destination(dv_, v, "dv", zero_all);
+  if (diff) {
+    diff->dlam = torch::empty_like(diff->lam, diff->lam.options(), at::MemoryFormat::Contiguous);
+    if (empty) diff->dlam.zero_();
+  }
   if (empty) return {dq, dk, dv};
 
   FaBwdParams p = {};
@@ -300,12 +417,50 @@ std::vector<at::Tensor> mha_varlen_bwd(at::Tensor q, at::Tensor k, at::Tensor v,
   p.cu_seqlens_q = cu_seqlens_q.data_ptr<int>();
   p.cu_seqlens_k = cu_seqlens_k.data_ptr<int>();
   p.flags = bwd_flags | (zero_all ? 0 : FA_BWD_ZERO_UNUSED_ROWS);
-  const size_t ws = fa_bwd_workspace_bytes(&p);
-  at::Tensor workspace = torch::empty({static_cast<int64_t>(ws)}, q.options().dtype(torch::kUInt8));
-  p.workspace = workspace.data_ptr();
-  p.workspace_bytes = ws;
-  check_rc(fa_bwd(&p, current_stream()), "fa_bwd");
+  launch_backward(p, diff, q, num_heads);
   return {dq, dk, dv};
+}
+
+std::vector<at::Tensor> mha_varlen_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor l,
+                                       at::Tensor dout, at::Tensor cu_seqlens_q, at::Tensor cu_seqlens_k,
+                                       const int64_t max_seqlen_q, const int64_t max_seqlen_k,
+                                       const double softmax_scale, bool is_causal,
+                                       c10::optional<at::Tensor> dq_, c10::optional<at::Tensor> dk_,
+                                       c10::optional<at::Tensor> dv_) {
+  return varlen_backward(q, k, v, out, l, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal,
+                         dq_, dk_, dv_, nullptr);
+}
+
+// ---- differential attention, without an autograd node: (out, lse, o2 when keep) and (dq, dk, dv, dlam) ----
+std::vector<at::Tensor> diff_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor lam, double softmax_scale, bool is_causal, bool keep) {
+  Differential diff{lam, keep, {}, {}};
+  auto r = dense_forward(q, k, v, softmax_scale, is_causal, c10::nullopt, c10::nullopt, c10::nullopt, &diff);
+  if (keep) r.push_back(diff.o2);
+  return r;
+}
+std::vector<at::Tensor> diff_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor lam, at::Tensor out, at::Tensor o2, at::Tensor l,
+                                 at::Tensor dout, double softmax_scale, bool is_causal) {
+  Differential diff{lam, true, o2, {}};
+  auto r = dense_backward(q, k, v, out, l, dout, softmax_scale, is_causal, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, &diff);
+  r.push_back(diff.dlam);
+  return r;
+}
+std::vector<at::Tensor> diff_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor lam, at::Tensor cu_seqlens_q,
+                                        at::Tensor cu_seqlens_k, int64_t max_seqlen_q, int64_t max_seqlen_k, double softmax_scale,
+                                        bool is_causal, bool keep) {
+  Differential diff{lam, keep, {}, {}};
+  auto r = varlen_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal, &diff);
+  if (keep) r.push_back(diff.o2);
+  return r;
+}
+std::vector<at::Tensor> diff_varlen_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor lam, at::Tensor out, at::Tensor o2,
+                                        at::Tensor l, at::Tensor dout, at::Tensor cu_seqlens_q, at::Tensor cu_seqlens_k,
+                                        int64_t max_seqlen_q, int64_t max_seqlen_k, double softmax_scale, bool is_causal) {
+  Differential diff{lam, true, o2, {}};
+  auto r = varlen_backward(q, k, v, out, l, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, is_causal,
+                           c10::nullopt, c10::nullopt, c10::nullopt, &diff);
+  r.push_back(diff.dlam);
+  return r;
 }
 
 // ---- the public dense and varlen functions in one call (flash_attention_interface.py) ----
@@ -340,7 +495,11 @@ bool plain_scale(const py::object& o, int64_t d, double& scale) {
   return true;
 }
 
-at::Tensor last_dim_contiguous(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+at::Tensor last_dim_contiguous(const at::Tensor& t) {
+  if (t.stride(-1) == 1) return t;
+  // an empty expanded tensor (the gradient of a sum, say) counts as contiguous whatever its strides
+  return t.numel() == 0 ? torch::empty(t.sizes(), t.options()) : t.contiguous();
+}
 
 struct Call {
   int64_t layout, max_q, max_k;
@@ -364,24 +523,26 @@ Qkv unpack(const Call& c, const at::Tensor& a, const at::Tensor& b, const at::Te
   return {a, b, d};
 }
 
-std::vector<at::Tensor> attend(const Call& c, const Qkv& x, const at::Tensor& cu_q, const at::Tensor& cu_k) {
+// diff: differential attention, and what it has besides q, k and v
+std::vector<at::Tensor> attend(const Call& c, const Qkv& x, const at::Tensor& cu_q, const at::Tensor& cu_k, Differential* diff) {
   const at::Tensor q = last_dim_contiguous(x.q), k = last_dim_contiguous(x.k), v = last_dim_contiguous(x.v);
-  if (c.varlen) return mha_varlen_fwd(q, k, v, cu_q, cu_k, c.max_q, c.max_k, c.scale, c.causal);
-  return mha_fwd(q, k, v, c.scale, c.causal, c10::nullopt, c10::nullopt, c10::nullopt);
+  if (c.varlen) return varlen_forward(q, k, v, cu_q, cu_k, c.max_q, c.max_k, c.scale, c.causal, diff);
+  return dense_forward(q, k, v, c.scale, c.causal, c10::nullopt, c10::nullopt, c10::nullopt, diff);
 }
 
 struct Attention : public torch::autograd::Function<Attention> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const Call& c, const at::Tensor& a,
                             const c10::optional<at::Tensor>& b, const c10::optional<at::Tensor>& d,
-                            const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k) {
+                            const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
+                            const c10::optional<at::Tensor>& lam) {
     const at::Tensor none;
     const Qkv x = unpack(c, a, b.value_or(none), d.value_or(none));
-    auto out = attend(c, x, cu_q.value_or(none), cu_k.value_or(none));
-    if (c.varlen) {
-      ctx->save_for_backward({x.q, x.k, x.v, out[0], out[1], *cu_q, *cu_k});
-    } else {
-      ctx->save_for_backward({x.q, x.k, x.v, out[0], out[1]});
-    }
+    Differential diff{lam.value_or(none), true, {}, {}};
+    auto out = attend(c, x, cu_q.value_or(none), cu_k.value_or(none), lam.has_value() ? &diff : nullptr);
+    torch::autograd::variable_list saved{x.q, x.k, x.v, out[0], out[1]};
+    if (c.varlen) saved.insert(saved.end(), {*cu_q, *cu_k});
+    if (lam.has_value()) saved.insert(saved.end(), {*lam, diff.o2});
+    ctx->save_for_backward(std::move(saved));
     auto& data = ctx->saved_data;
     data["layout"] = c.layout, data["max_q"] = c.max_q, data["max_k"] = c.max_k;
     data["varlen"] = c.varlen, data["causal"] = c.causal, data["scale"] = c.scale;
@@ -412,24 +573,31 @@ struct Attention : public torch::autograd::Function<Attention> {
       auto parts = packed.unbind(dim);
       dq = at::empty_like(q), dk = parts[0], dv = parts[1];
     }
+    const size_t extra = c.varlen ? 7 : 5;  // lam and A_2 V of differential attention
+    Differential diff;
+    if (saved.size() > extra) diff = Differential{saved[extra], true, saved[extra + 1], {}};
+    Differential* which = saved.size() > extra ? &diff : nullptr;
     const at::Tensor dout = last_dim_contiguous(grads[0]), out = last_dim_contiguous(saved[3]), lse = last_dim_contiguous(saved[4]);
     const at::Tensor cq = last_dim_contiguous(q), ck = last_dim_contiguous(k), cv = last_dim_contiguous(v);
-    auto g = c.varlen ? mha_varlen_bwd(cq, ck, cv, out, lse, dout, saved[5], saved[6], c.max_q, c.max_k, c.scale, c.causal, dq, dk, dv)
-                      : mha_bwd(cq, ck, cv, out, lse, dout, c.scale, c.causal, dq, dk, dv, c10::nullopt);
+    auto g = c.varlen ? varlen_backward(cq, ck, cv, out, lse, dout, saved[5], saved[6], c.max_q, c.max_k, c.scale, c.causal, dq, dk, dv, which)
+                      : dense_backward(cq, ck, cv, out, lse, dout, c.scale, c.causal, dq, dk, dv, c10::nullopt, which);
     const at::Tensor none;  // one entry per argument of forward()
-    if (c.layout == kQkvPacked) return {none, packed, none, none, none, none};
-    if (c.layout == kKvPacked) return {none, g[0], packed, none, none, none};
-    return {none, g[0], g[1], g[2], none, none};
+    if (c.layout == kQkvPacked) return {none, packed, none, none, none, none, none};
+    if (c.layout == kKvPacked) return {none, g[0], packed, none, none, none, none};
+    return {none, g[0], g[1], g[2], none, none, diff.dlam};
   }
 };
 
 py::object attention(const Call& c, const at::Tensor& a, const c10::optional<at::Tensor>& b, const c10::optional<at::Tensor>& d,
-                     const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k) {
-  const bool needs_grad = at::GradMode::is_enabled() &&
-                          (a.requires_grad() || (b.has_value() && b->requires_grad()) || (d.has_value() && d->requires_grad()));
-  if (needs_grad) return py::cast(Attention::apply(c, a, b, d, cu_q, cu_k));
+                     const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
+                     const c10::optional<at::Tensor>& lam = c10::nullopt) {
+  auto wants = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  const bool needs_grad = at::GradMode::is_enabled() && (a.requires_grad() || wants(b) || wants(d) || wants(lam));
+  if (needs_grad) return py::cast(Attention::apply(c, a, b, d, cu_q, cu_k, lam));
   const at::Tensor none;
-  return py::cast(attend(c, unpack(c, a, b.value_or(none), d.value_or(none)), cu_q.value_or(none), cu_k.value_or(none))[0]);
+  Differential diff{lam.value_or(none), false, {}, {}};
+  return py::cast(attend(c, unpack(c, a, b.value_or(none), d.value_or(none)), cu_q.value_or(none), cu_k.value_or(none),
+                         lam.has_value() ? &diff : nullptr)[0]);
 }
 
 // The tensors of a layout: (q, k, v), (q, kv, None) or (qkv, None, None).
@@ -446,19 +614,28 @@ bool plain_inputs(int64_t layout, int64_t dim, const py::object& a, const py::ob
   return true;
 }
 
-py::object attention_dense(int64_t layout, py::object a, py::object b, py::object d, py::object softmax_scale, py::object causal) {
-  at::Tensor ta;
-  c10::optional<at::Tensor> tb, td;
-  Call c{layout, 0, 0, false, causal.ptr() == Py_True, 0.0};
-  if (!plain_eager() || !PyBool_Check(causal.ptr()) || !plain_inputs(layout, 4, a, b, d, ta, tb, td) ||
-      !plain_scale(softmax_scale, ta.size(-1), c.scale))
-    return py::none();
-  return attention(c, ta, tb, td, c10::nullopt, c10::nullopt);
+// The weights of differential attention: an ordinary tensor of any shape and type, which are checked later
+bool plain_lam(const py::object& o, at::Tensor& t) {
+  if (!THPVariable_CheckExact(o.ptr())) return false;
+  t = THPVariable_Unpack(o.ptr());
+  return !t._fw_grad(/*level=*/0).defined();
 }
 
-py::object attention_varlen(int64_t layout, py::object a, py::object b, py::object d, py::object cu_q, py::object cu_k, py::object max_q,
-                            py::object max_k, py::object softmax_scale, py::object causal) {
-  at::Tensor ta;
+// lam: None, or the weights of differential attention, whose maps have half of the head dimension each
+py::object dense_call(int64_t layout, py::object a, py::object b, py::object d, py::object lam, py::object softmax_scale, py::object causal) {
+  at::Tensor ta, tl;
+  c10::optional<at::Tensor> tb, td;
+  Call c{layout, 0, 0, false, causal.ptr() == Py_True, 0.0};
+  const bool diff = !lam.is_none();
+  if (!plain_eager() || !PyBool_Check(causal.ptr()) || !plain_inputs(layout, 4, a, b, d, ta, tb, td) ||
+      !plain_scale(softmax_scale, diff ? ta.size(-1) / 2 : ta.size(-1), c.scale) || (diff && !plain_lam(lam, tl)))
+    return py::none();
+  return attention(c, ta, tb, td, c10::nullopt, c10::nullopt, diff ? c10::optional<at::Tensor>(tl) : c10::nullopt);
+}
+
+py::object varlen_call(int64_t layout, py::object a, py::object b, py::object d, py::object lam, py::object cu_q, py::object cu_k,
+                       py::object max_q, py::object max_k, py::object softmax_scale, py::object causal) {
+  at::Tensor ta, tl;
   c10::optional<at::Tensor> tb, td;
   Call c{layout, 0, 0, true, causal.ptr() == Py_True, 0.0};
   auto index = [](const py::object& o, int64_t& value) {
@@ -467,11 +644,28 @@ py::object attention_varlen(int64_t layout, py::object a, py::object b, py::obje
     value = PyLong_AsLongLongAndOverflow(o.ptr(), &overflow);
     return overflow == 0;
   };
+  const bool diff = !lam.is_none();
   if (!plain_eager() || !PyBool_Check(causal.ptr()) || !plain_inputs(layout, 3, a, b, d, ta, tb, td) ||
-      !plain_scale(softmax_scale, ta.size(-1), c.scale) || !THPVariable_CheckExact(cu_q.ptr()) || !THPVariable_CheckExact(cu_k.ptr()) ||
-      !index(max_q, c.max_q) || !index(max_k, c.max_k))
+      !plain_scale(softmax_scale, diff ? ta.size(-1) / 2 : ta.size(-1), c.scale) || !THPVariable_CheckExact(cu_q.ptr()) ||
+      !THPVariable_CheckExact(cu_k.ptr()) || !index(max_q, c.max_q) || !index(max_k, c.max_k) || (diff && !plain_lam(lam, tl)))
     return py::none();
-  return attention(c, ta, tb, td, THPVariable_Unpack(cu_q.ptr()), THPVariable_Unpack(cu_k.ptr()));
+  return attention(c, ta, tb, td, THPVariable_Unpack(cu_q.ptr()), THPVariable_Unpack(cu_k.ptr()),
+                   diff ? c10::optional<at::Tensor>(tl) : c10::nullopt);
+}
+
+py::object attention_dense(int64_t layout, py::object a, py::object b, py::object d, py::object softmax_scale, py::object causal) {
+  return dense_call(layout, a, b, d, py::none(), softmax_scale, causal);
+}
+py::object attention_varlen(int64_t layout, py::object a, py::object b, py::object d, py::object cu_q, py::object cu_k, py::object max_q,
+                            py::object max_k, py::object softmax_scale, py::object causal) {
+  return varlen_call(layout, a, b, d, py::none(), cu_q, cu_k, max_q, max_k, softmax_scale, causal);
+}
+py::object diff_attention_dense(py::object q, py::object k, py::object v, py::object lam, py::object softmax_scale, py::object causal) {
+  return dense_call(kSeparate, q, k, v, lam, softmax_scale, causal);
+}
+py::object diff_attention_varlen(py::object q, py::object k, py::object v, py::object lam, py::object cu_q, py::object cu_k,
+                                 py::object max_q, py::object max_k, py::object softmax_scale, py::object causal) {
+  return varlen_call(kSeparate, q, k, v, lam, cu_q, cu_k, max_q, max_k, softmax_scale, causal);
 }
 
 // The word of pinned host memory in which the device answers fa_kvcache_checked(): one per thread, which waits for its answer
@@ -527,7 +721,7 @@ std::vector<at::Tensor> kvcache_forward(Verdict* checked, at::Tensor q, at::Tens
                                         py::object alibi_slopes_obj, py::object out_obj,
                                         const double softmax_scale, bool is_causal, int64_t window_size_left,
                                         int64_t window_size_right, const double softcap,
-                                        bool rotary_interleaved, int64_t num_splits) {
+                                        bool rotary_interleaved, int64_t num_splits, const at::Tensor* lam = nullptr) {
   (void)rotary_interleaved;
   TORCH_CHECK(rotary_cos_obj.is_none() && rotary_sin_obj.is_none(),
               "Turing KV-cache does not support rotary embeddings yet");
@@ -617,10 +811,16 @@ std::vector<at::Tensor> kvcache_forward(Verdict* checked, at::Tensor q, at::Tens
     TORCH_CHECK(k.stride(-1) == 1 && v.stride(-1) == 1, "k and v must have contiguous last dimension");
     seqlen_new = k.size(1);
   }
+  if (lam) {
+    check_same_device(q, {k_cache, v_cache, cache_seqlens});
+    if (has_k) check_same_device(q, {k, v});
+    if (has_block_table) check_same_device(q, {block_table});
+    diff_weights(*lam, q, num_heads);
+  }
   c10::cuda::CUDAGuard guard(q.device());
 
   at::Tensor out = torch::empty_like(q, q.options(), at::MemoryFormat::Contiguous);
-  at::Tensor lse = torch::empty({batch_size, num_heads, seqlen_q}, q.options().dtype(torch::kFloat32));
+  at::Tensor lse = torch::empty({batch_size, lam ? 2 * num_heads : num_heads, seqlen_q}, q.options().dtype(torch::kFloat32));
   if (batch_size == 0 || seqlen_q == 0) return {out, lse};
 
   FaKvcacheParams p = {};
@@ -649,16 +849,22 @@ std::vector<at::Tensor> kvcache_forward(Verdict* checked, at::Tensor q, at::Tens
     p.max_blocks_per_seq = block_table.size(1);
   }
   p.num_splits = static_cast<int32_t>(num_splits);
-  const size_t ws = fa_kvcache_workspace_bytes(&p);
-  at::Tensor workspace = torch::empty({static_cast<int64_t>(ws)}, q.options().dtype(torch::kUInt8));
+  FaDiffKvcacheParams dp = {};
+  if (lam) dp.base = p, dp.weights = diff_weights(*lam, q, num_heads);
+  const size_t ws = lam ? fa_diff_kvcache_workspace_bytes(&dp) : fa_kvcache_workspace_bytes(&p);
+  at::Tensor workspace = scratch(ws, q);
   p.workspace = ws ? workspace.data_ptr() : nullptr;
   p.workspace_bytes = ws;
+  dp.base.workspace = p.workspace, dp.base.workspace_bytes = ws;
   if (checked) {
     checked->next();
-    const int rc = fa_kvcache_checked(&p, checked->word, checked->token, current_stream());
+    const int rc = lam ? fa_diff_kvcache(&dp, checked->word, checked->token, current_stream())
+                       : fa_kvcache_checked(&p, checked->word, checked->token, current_stream());
     checked->refused_by_host = rc != FA_ERR_CUDA;
     if (rc != FA_OK) checked->settle(at::cuda::getCurrentCUDAStream().stream());
-    check_rc(rc, "fa_kvcache_checked");
+    check_rc(rc, lam ? "fa_diff_kvcache" : "fa_kvcache_checked");
+  } else if (lam) {
+    check_rc(fa_diff_kvcache(&dp, nullptr, 0, current_stream()), "fa_diff_kvcache");
   } else {
     check_rc(fa_kvcache(&p, current_stream()), "fa_kvcache");
   }
@@ -682,9 +888,9 @@ std::vector<at::Tensor> mha_fwd_kvcache(at::Tensor q, at::Tensor k_cache, at::Te
 // launched first and the answer is waited for under them.  None when the call has to be checked beforehand: no work to
 // launch, a stream that is being captured, or arguments that are refused (a capacity that is insufficient is told of first, whatever
 // else is wrong).  What fails in a launch or on the device is an error of this call.
-py::object fwd_kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, py::object k, py::object v,
-                               at::Tensor cache_seqlens, py::object cache_batch_idx, py::object block_table,
-                               double softmax_scale, bool is_causal, int64_t num_splits) {
+py::object kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, py::object k, py::object v,
+                           at::Tensor cache_seqlens, py::object cache_batch_idx, py::object block_table,
+                           double softmax_scale, bool is_causal, int64_t num_splits, const at::Tensor* lam) {
   if (!q.is_cuda() || q.numel() == 0 || cache_seqlens.device() != q.device()) return py::none();
   c10::cuda::CUDAGuard guard(q.device());
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -696,7 +902,7 @@ py::object fwd_kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_ca
   verdict.refused_by_host = true;
   try {
     r = kvcache_forward(&verdict, q, k_cache, v_cache, k, v, cache_seqlens, py::none(), py::none(), cache_batch_idx, py::none(),
-                        block_table, py::none(), py::none(), softmax_scale, is_causal, -1, -1, 0.0, true, num_splits);
+                        block_table, py::none(), py::none(), softmax_scale, is_causal, -1, -1, 0.0, true, num_splits, lam);
   } catch (const std::exception&) {
     if (!verdict.refused_by_host) throw;
     return py::none();
@@ -707,6 +913,26 @@ py::object fwd_kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_ca
     fits = verdict.wait(stream);
   }
   return py::make_tuple(r[0], r[1], fits);
+}
+
+py::object fwd_kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, py::object k, py::object v,
+                               at::Tensor cache_seqlens, py::object cache_batch_idx, py::object block_table,
+                               double softmax_scale, bool is_causal, int64_t num_splits) {
+  return kvcache_checked(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, is_causal, num_splits,
+                         nullptr);
+}
+
+// Differential attention against a KV cache: checked as above, and without the check
+py::object diff_kvcache_checked(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor lam, py::object k, py::object v,
+                                at::Tensor cache_seqlens, py::object cache_batch_idx, py::object block_table, double softmax_scale,
+                                bool is_causal, int64_t num_splits) {
+  return kvcache_checked(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, is_causal, num_splits, &lam);
+}
+std::vector<at::Tensor> diff_kvcache(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor lam, py::object k, py::object v,
+                                     at::Tensor cache_seqlens, py::object cache_batch_idx, py::object block_table, double softmax_scale,
+                                     bool is_causal, int64_t num_splits) {
+  return kvcache_forward(nullptr, q, k_cache, v_cache, k, v, cache_seqlens, py::none(), py::none(), cache_batch_idx, py::none(), block_table,
+                         py::none(), py::none(), softmax_scale, is_causal, -1, -1, 0.0, true, num_splits, &lam);
 }
 
 // ---- stand-alone LSE merge (no counterpart binding in the reference; used after the NCCL exchange
@@ -828,6 +1054,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dq") = py::none(), py::arg("dk") = py::none(), py::arg("dv") = py::none());
   m.def("fwd_kvcache", &mha_fwd_kvcache, "KV-cache forward pass");
   m.def("fwd_kvcache_checked", &fwd_kvcache_checked, "KV-cache forward pass that refuses lengths beyond the capacity");
+  m.def("diff_attention_dense", &diff_attention_dense, "Differential attention with its autograd node; None: for the autograd.Function class");
+  m.def("diff_attention_varlen", &diff_attention_varlen, "The same for packed sequences");
+  m.def("diff_fwd", &diff_fwd, "Differential attention: out, lse of both maps and, with keep, the second map's output");
+  m.def("diff_bwd", &diff_bwd, "Its backward: dq, dk, dv, dlam");
+  m.def("diff_varlen_fwd", &diff_varlen_fwd, "Packed differential attention");
+  m.def("diff_varlen_bwd", &diff_varlen_bwd, "Its backward");
+  m.def("diff_kvcache", &diff_kvcache, "Differential attention against a KV cache");
+  m.def("diff_kvcache_checked", &diff_kvcache_checked, "The same, refusing lengths beyond the capacity");
   m.def("kvcache_answer_words", [] { return g_verdict_words.load(); },
         "Pinned words that fwd_kvcache_checked holds: one per thread that called it and is alive");
   m.def("combine", &combine, "Merge split partials (O fp32, LSE) with log-sum-exp weights");

@@ -1,0 +1,106 @@
+"""Differential attention: the difference of two softmax maps with a learned weight per head.
+
+The halves of the head dimension of q and k give two maps over the same values::
+
+    A_m = softmax(scale * Q_m K_m^T [+ causal mask]),  m = 1, 2        out = (A_1 - lam_h * A_2) V
+
+Shapes, masks (bottom-right aligned), grouped heads, packed sequences and the KV cache are those of ``flash_attn_func``,
+``flash_attn_varlen_func`` and ``flash_attn_with_kvcache``: fp16, head dimension 64 or 128 (maps of 32 or 64).  A model that keeps
+2 * nheads query heads of d / 2 and values of d passes ``q.view(b, s, nheads, d)``: the two maps of a head lie next to each other.
+``lam`` holds one weight per query head, or a single one for all, fp32 or fp16, and has a gradient.  What a model puts around the
+operator (how lam is parametrised, a norm of the heads' outputs) is its own.
+No counterpart in Cy-47/flash-attention-turing.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from .flash_attention_interface import _diff_scale, _gpu, _kvcache_step, maybe_contiguous
+
+
+# The classes answer what the native autograd node leaves to them: functorch transforms, tracing, modes, tensor subclasses,
+# forward-mode AD, and inputs that are refused.
+class FlashDiffAttnFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, softmax_scale, causal, is_grad_enabled):
+        scale = _diff_scale(q, softmax_scale)
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        keep = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        out, lse, *o2 = _gpu().diff_fwd(q, k, v, lam, scale, causal, keep)
+        if keep:
+            ctx.save_for_backward(q, k, v, lam, out, *o2, lse)
+            ctx.softmax_scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, lam, out, o2, lse = ctx.saved_tensors
+        dq, dk, dv, dlam = _gpu().diff_bwd(q, k, v, lam, out, o2, lse, maybe_contiguous(dout), ctx.softmax_scale, ctx.causal)
+        return dq, dk, dv, dlam, None, None, None
+
+
+class FlashDiffAttnVarlenFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
+                is_grad_enabled):
+        scale = _diff_scale(q, softmax_scale)
+        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        keep = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
+        out, lse, *o2 = _gpu().diff_varlen_fwd(q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, keep)
+        if keep:
+            ctx.save_for_backward(q, k, v, lam, out, *o2, lse, cu_seqlens_q, cu_seqlens_k)
+            ctx.lengths = max_seqlen_q, max_seqlen_k
+            ctx.softmax_scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, lam, out, o2, lse, cu_q, cu_k = ctx.saved_tensors
+        dq, dk, dv, dlam = _gpu().diff_varlen_bwd(q, k, v, lam, out, o2, lse, maybe_contiguous(dout), cu_q, cu_k, *ctx.lengths,
+                                                  ctx.softmax_scale, ctx.causal)
+        return dq, dk, dv, dlam, None, None, None, None, None, None, None
+
+
+def flash_diff_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                         softmax_scale: Optional[float] = None, causal: bool = False) -> torch.Tensor:
+    """q (batch, seqlen_q, nheads, d); k, v (batch, seqlen_k, nheads_k, d); lam (nheads,) or one element -> out like q.
+    ``softmax_scale`` defaults to (d / 2) ** -0.5.  Differentiable in q, k, v and lam; every gradient is bitwise reproducible."""
+    out = _gpu().diff_attention_dense(q, k, v, lam, softmax_scale, causal)
+    return FlashDiffAttnFunc.apply(q, k, v, lam, softmax_scale, causal, torch.is_grad_enabled()) if out is None else out
+
+
+def flash_diff_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                                cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                                softmax_scale: Optional[float] = None, causal: bool = False) -> torch.Tensor:
+    """Packed sequences: q (total_q, nheads, d); k, v (total_k, nheads_k, d); cu_seqlens_* int32 (batch + 1,) -> out like q.
+    Rows outside every sequence are zero in the output and in the gradients and count for nothing."""
+    out = _gpu().diff_attention_varlen(q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal)
+    if out is not None:
+        return out
+    return FlashDiffAttnVarlenFunc.apply(q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                                         causal, torch.is_grad_enabled())
+
+
+def flash_diff_attn_with_kvcache(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    lam: torch.Tensor,
+    k: Optional[torch.Tensor] = None,
+    v: Optional[torch.Tensor] = None,
+    cache_seqlens: Optional[Union[torch.Tensor, int]] = None,
+    cache_batch_idx: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    causal: bool = False,
+    num_splits: int = 0,
+) -> torch.Tensor:
+    """Inference step against a KV cache: appends ``k``/``v`` in place at ``cache_seqlens`` and attends ``q`` against the first
+    ``cache_seqlens + seqlen_new`` tokens.  The caches (contiguous or paged), the arguments and their checks are those of
+    ``flash_attn_with_kvcache``, and a cache may be used by both.  Not differentiable."""
+    if not isinstance(lam, torch.Tensor):
+        raise TypeError("lam must be a torch.Tensor")
+    return _kvcache_step(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, causal, num_splits,
+                         False, lam=lam)

@@ -47,6 +47,11 @@ def _default_scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
     return q.shape[-1] ** (-0.5) if softmax_scale is None else softmax_scale
 
 
+def _diff_scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
+    """Differential attention: each of the two maps has half of the head dimension."""
+    return (q.shape[-1] // 2) ** (-0.5) if softmax_scale is None else softmax_scale
+
+
 # --------------------------------------------------------------------------------------------
 # thin wrappers around the five bindings (reference :13-169)
 # --------------------------------------------------------------------------------------------
@@ -81,11 +86,15 @@ def _flash_attn_varlen_backward(dout, q, k, v, out, lse, cu_seqlens_q, cu_seqlen
 
 
 def _flash_attn_kvcache_forward(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table,
-                                softmax_scale: float, causal: bool, num_splits: int, checked: bool = False):
-    """``checked``: (out, lse, whether all lengths fit the cache), or None when that has to be found out beforehand."""
+                                softmax_scale: float, causal: bool, num_splits: int, checked: bool = False, lam=None):
+    """``checked``: (out, lse, whether all lengths fit the cache), or None when that has to be found out beforehand.
+    ``lam``: the weights of differential attention."""
     q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table = (
         maybe_contiguous(t) for t in (q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table)
     )
+    if lam is not None:
+        step = _gpu().diff_kvcache_checked if checked else _gpu().diff_kvcache
+        return step(q, k_cache, v_cache, lam, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, causal, num_splits)
     if checked:
         return _gpu().fwd_kvcache_checked(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table,
                                           softmax_scale, causal, num_splits)
@@ -370,6 +379,13 @@ def flash_attn_with_kvcache(
     Returns ``out`` or ``(out, softmax_lse)``.
     """
     _validate_unsupported_kvcache_args(rotary_cos, rotary_sin, cache_leftpad, window_size, softcap, alibi_slopes)
+    return _kvcache_step(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table,
+                         softmax_scale, causal, num_splits, return_softmax_lse)
+
+
+def _kvcache_step(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, softmax_scale, causal, num_splits,
+                  return_softmax_lse, lam=None):
+    """The checks and the call behind ``flash_attn_with_kvcache`` and, with ``lam``, ``flash_diff_attn_with_kvcache``."""
     if (k is None) != (v is None):
         raise ValueError("k and v must either both be provided or both be None")
     _validate_supported_head_dim(q.shape[-1])
@@ -413,10 +429,10 @@ def flash_attn_with_kvcache(
         seqlen_new = k.shape[1]
     # Capacity is checked before the device/dtype checks, on whatever device the lengths live
     # (the reference does the same, :855-858, and its tests rely on that order with CPU tensors).
-    scale = _default_scale(q, softmax_scale)
+    scale = _default_scale(q, softmax_scale) if lam is None else _diff_scale(q, softmax_scale)
     if HOST_CAPACITY_CHECK and cache_batch_idx is None and all(t.is_cuda for t in (q, k_cache, v_cache, cache_seqlens)):
         r = _flash_attn_kvcache_forward(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx, block_table, scale,
-                                        causal, num_splits, checked=True)
+                                        causal, num_splits, checked=True, lam=lam)
         if r is not None:
             out, lse, fits = r
             if not fits:
@@ -438,5 +454,5 @@ def flash_attn_with_kvcache(
             raise RuntimeError("k and v must be float16 tensors")
 
     out, lse = _flash_attn_kvcache_forward(q, k_cache, v_cache, k, v, cache_seqlens, cache_batch_idx,
-                                           block_table, scale, causal, num_splits)
+                                           block_table, scale, causal, num_splits, lam=lam)
     return (out, lse) if return_softmax_lse else out

@@ -349,6 +349,59 @@ typedef struct FaSumGatherParams {
 
 int fa_sum_gather(const FaSumGatherParams* p, fa_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------- */
+/* Differential attention: the halves of head_dim of q and k give two softmax maps over the same  */
+/* values, A_m = softmax(Q_m K_m^T * scale [+ causal mask]) for m = 1, 2, and                     */
+/*   O = (A_1 - lam_h A_2) V                                                                     */
+/* with a learned weight lam_h per query head.  Shapes, masks and strides are those of the calls   */
+/* above (`base`), with these differences: q and k are cut in two along d (softmax_scale is applied */
+/* as given, (d / 2)^-1/2 is usual); base.lse holds two rows per head, (b, 2 * h, lse_row_stride),   */
+/* row 2 * head + map; a row without a visible key gets O = 0 and both LSE = 0.  No counterpart in   */
+/* the reference.                                                                                 */
+/* ------------------------------------------------------------------------------------------- */
+typedef struct FaDiffWeights {
+  const void* lam;    /* fp32 or fp16                                                            */
+  int64_t stride;     /* elements between the weights of consecutive heads                       */
+  int32_t count;      /* h, or 1: one weight for all heads                                       */
+  int32_t is_half;    /* 0: fp32, 1: fp16                                                        */
+} FaDiffWeights;
+
+typedef struct FaDiffFwdParams {
+  FaFwdParams base;   /* seqused_k, block_table and FA_CAUSAL_SHIFT included                     */
+  FaDiffWeights weights;
+  void* o2;           /* NULL, or A_2 V (fp16, the shape of o, its own strides): fa_diff_bwd() needs it */
+  int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
+  void* workspace;    /* 256-byte aligned, fa_diff_fwd_workspace_bytes() bytes                    */
+  size_t workspace_bytes;
+} FaDiffFwdParams;
+
+size_t fa_diff_fwd_workspace_bytes(const FaDiffFwdParams* p);
+int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream);
+
+/* Backward: dq, dk, dv (per KV head, summed over its query heads) and the gradient of the weights. */
+/* base.flags: 0 or FA_BWD_ZERO_UNUSED_ROWS; base.workspace holds fa_diff_bwd_workspace_bytes().   */
+/* Every gradient is bitwise reproducible.  dk and dv must not lie over k and v.                   */
+typedef struct FaDiffBwdParams {
+  FaBwdParams base;   /* o, lse: what fa_diff_fwd() wrote                                        */
+  FaDiffWeights weights;
+  const void* o2;
+  int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
+  void* dlam;         /* weights.count gradients (1: summed over the heads), contiguous, of the type of lam */
+} FaDiffBwdParams;
+
+size_t fa_diff_bwd_workspace_bytes(const FaDiffBwdParams* p);
+int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream);
+
+/* KV-cache step: append, then attend as in fa_kvcache(), with the same cache.  base.lse: (b, 2 * h, seqlen_q).  verdict and  */
+/* token as in fa_kvcache_checked(), or verdict == NULL: lengths beyond the capacity are clamped.                       */
+typedef struct FaDiffKvcacheParams {
+  FaKvcacheParams base;
+  FaDiffWeights weights;
+} FaDiffKvcacheParams;
+
+size_t fa_diff_kvcache_workspace_bytes(const FaDiffKvcacheParams* p);
+int fa_diff_kvcache(const FaDiffKvcacheParams* p, int32_t* verdict, int32_t token, fa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
