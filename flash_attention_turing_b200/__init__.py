@@ -18,6 +18,13 @@ from .diff_attention_interface import (  # noqa: F401
     flash_diff_attn_varlen_func,
     flash_diff_attn_with_kvcache,
 )
+from .kvcache_pages import (  # noqa: F401
+    kvcache_compact,
+    kvcache_copy_pages,
+    kvcache_fork,
+    kvcache_free,
+    kvcache_reserve,
+)
 
 
 
@@ -62,4 +69,9 @@ __all__ = [
     "flash_diff_attn_func",
     "flash_diff_attn_varlen_func",
     "flash_diff_attn_with_kvcache",
+    "kvcache_compact",
+    "kvcache_copy_pages",
+    "kvcache_fork",
+    "kvcache_free",
+    "kvcache_reserve",
 ]

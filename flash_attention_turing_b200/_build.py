@@ -2,7 +2,7 @@
 
 * ``libfa_b200.so``   -- the C-ABI launcher library (``include/fa_b200.h``): hand-written sm_100a
   kernels compiled with ``nvcc -gencode arch=compute_100a,code=sm_100a``; no torch dependency.
-* ``_fa_b200_torch*.so`` -- the thin PyTorch binding (``csrc/torch_ext.cpp``) that mirrors the five
+* ``_fa_b200_torch*.so`` -- the thin PyTorch binding (``csrc/torch_ext*.cpp``) that mirrors the five
   functions of the reference extension (``csrc/flash_attn/flash_api.cpp:717-724`` in
   Cy-47/flash-attention-turing) and links against ``libfa_b200.so``.
 
@@ -29,7 +29,8 @@ EXT_NAME = "_fa_b200_torch"
 EXT_PATH = PKG_DIR / f"{EXT_NAME}.so"
 
 CUDA_SOURCES = ["common.cu", "fwd_sm100.cu", "bwd_sm100.cu", "bwd_fused_sm100.cu", "kvcache_sm100.cu", "combine.cu",
-                "diff.cu"]
+                "diff.cu", "kvcache_pages.cu"]
+BINDING_SOURCES = ["torch_ext.cpp", "torch_ext_pages.cpp"]
 # Ahead of the compiler's own -lstdc++, which is an archive in some installations: a second C++ runtime in the extension takes the
 # place of a part of the one torch uses, and formatting a number for an exception then crashes the process.
 CXX_RUNTIME = "-l:libstdc++.so.6"
@@ -96,33 +97,41 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_torch_extension(force: bool = False, verbose: bool = False) -> Path:
-    """Compile ``csrc/torch_ext.cpp`` with the host compiler against this torch install."""
+    """Compile the binding's sources with the host compiler against this torch install."""
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "torch_ext.cpp"
-    deps = [src, *INCLUDE.glob("*.h"), LIB_PATH]
+    common = [CSRC / "torch_common.h", *INCLUDE.glob("*.h")]
+    deps = [*(CSRC / src for src in BINDING_SOURCES), *common, LIB_PATH]
     stamp = OBJ_DIR / "torch_ext.stamp"
     tag = f"{torch.__version__}|{sys.version_info[:2]}|{CXX_RUNTIME}"
-    if not force and _newer(EXT_PATH, deps) and stamp.exists() and stamp.read_text() == tag:
+    same_tag = stamp.exists() and stamp.read_text() == tag
+    if not force and same_tag and _newer(EXT_PATH, deps):
         return EXT_PATH
     OBJ_DIR.mkdir(exist_ok=True)
     cuda_inc = _cuda_home() / "include"
     inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda_inc), str(INCLUDE)]
     torch_lib = cpp_extension.library_paths()[0]
     cxx11 = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [
-        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
-        f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-        f"-D_GLIBCXX_USE_CXX11_ABI={cxx11}",
-        *[f"-I{i}" for i in inc],
-        str(src), "-o", str(EXT_PATH),
+    cxx = os.environ.get("CXX", "g++")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-w", f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={cxx11}", *[f"-I{i}" for i in inc]]
+
+    def compile_one(src):
+        obj = OBJ_DIR / (src + ".o")
+        if force or not same_tag or not _newer(obj, [CSRC / src, *common]):
+            _run([cxx, *flags, "-c", str(CSRC / src), "-o", str(obj)])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(BINDING_SOURCES)) as pool:
+        objs = list(pool.map(compile_one, BINDING_SOURCES))
+    _run([
+        cxx, "-shared", *objs, "-o", str(EXT_PATH),
         CXX_RUNTIME,
         f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
         f"-L{PKG_DIR}", "-lfa_b200",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",
-    ]
-    _run(cmd)
+    ])
     stamp.write_text(tag)
     if verbose:
         print(f"[build] built {EXT_PATH.name}")

@@ -34,6 +34,12 @@ EXPORTED_SYMBOLS = (
     "fa_diff_bwd",
     "fa_diff_kvcache_workspace_bytes",
     "fa_diff_kvcache",
+    "fa_pages_workspace_bytes",
+    "fa_pages_reserve",
+    "fa_pages_fork",
+    "fa_pages_free",
+    "fa_pages_compact",
+    "fa_pages_copy",
 )
 
 _i64, _i32, _f32, _vp, _sz = C.c_int64, C.c_int32, C.c_float, C.c_void_p, C.c_size_t
@@ -103,6 +109,15 @@ class FaDiffKvcacheParams(C.Structure):
     _fields_ = [("base", FaKvcacheParams), ("weights", FaDiffWeights)]
 
 
+class FaPageTables(C.Structure):
+    _fields_ = [("block_table", _vp), ("cache_seqlens", _vp), ("page_refs", _vp), ("row_stride", _i64), ("rows", _i32),
+                ("columns", _i32), ("num_pages", _i32), ("reserved0", _i32)]
+
+
+class FaPageCaches(C.Structure):
+    _fields_ = [("base", C.POINTER(_vp)), ("page_stride", C.POINTER(_i64)), ("page_bytes", _i64), ("count", _i32), ("reserved0", _i32)]
+
+
 class FaCombineParams(C.Structure):
     _fields_ = [("o_accum", _vp), ("lse_accum", _vp), ("o", _vp), ("lse", _vp),
                 ("o_batch_stride", _i64), ("o_row_stride", _i64), ("o_head_stride", _i64),
@@ -166,6 +181,14 @@ def lib() -> C.CDLL:
             fn.restype, size.restype = C.c_int, _sz
             fn.argtypes = [C.POINTER(struct), _vp, _i32, _vp] if name == "fa_diff_kvcache" else [C.POINTER(struct), _vp]
             size.argtypes = [C.POINTER(struct)]
+        tables, caches = C.POINTER(FaPageTables), C.POINTER(FaPageCaches)
+        for name, args in (("reserve", [tables, _vp, _i32, _i32, _vp, _vp, _sz]), ("fork", [tables, caches, _vp, _vp, _i32, _i32, _vp, _vp, _sz]),
+                           ("free", [tables, _vp, _i32]), ("compact", [tables, caches, _vp, _vp, _sz]),
+                           ("copy", [caches, _i32, _vp, _vp, _i32, _vp, _vp, _sz])):
+            fn = getattr(l, "fa_pages_" + name)
+            fn.restype, fn.argtypes = C.c_int, [*args, _vp]
+        l.fa_pages_workspace_bytes.restype = _sz
+        l.fa_pages_workspace_bytes.argtypes = [_i32, _i32, _i32]
         l.fa_kvcache_num_splits.restype = C.c_int
         l.fa_kvcache_num_splits.argtypes = [C.POINTER(FaKvcacheParams)]
         _lib = l

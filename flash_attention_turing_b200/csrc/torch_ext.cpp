@@ -3,9 +3,7 @@
 // and checks.  This file only validates tensors, allocates outputs and scratch memory with the
 // torch caching allocator, fills the C-ABI parameter structs and calls the launcher on the current
 // CUDA stream of q's device.  It contains no kernels and has no CPU path.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
+#include "torch_common.h"
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -18,16 +16,9 @@
 #include <cmath>
 #include <vector>
 
-#include "../../include/fa_b200.h"
-
 namespace {
 
 std::atomic<int> g_bwd_flags{0};  // flags of FaBwdParams used by bwd / varlen_bwd (set_single_kernel_backward)
-
-
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == FA_OK, what, " failed (", rc, "): ", fa_last_error());
-}
 
 void check_supported_head_dim(int64_t d) {
   // message of check_supported_head_dim, flash_api.cpp:10-14
@@ -39,8 +30,6 @@ void check_half_cuda(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be a float16 tensor");
   TORCH_CHECK(t.stride(-1) == 1, name, " must have contiguous last dimension");
 }
-
-fa_stream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 // A log-sum-exp tensor (b, h, rows) given by the caller: fp32, unit stride along rows, heads of a batch one
 // row pitch apart -- e.g. a slice of the rows of a contiguous tensor.
@@ -75,11 +64,6 @@ FaDiffWeights diff_weights(const at::Tensor& lam, const at::Tensor& q, int64_t n
 
 void check_same_device(const at::Tensor& q, std::initializer_list<at::Tensor> others) {
   for (const at::Tensor& t : others) TORCH_CHECK(t.device() == q.device(), "all tensors must be on the device of q");
-}
-
-// Scratch memory of a call; 256-byte aligned, as the caching allocator gives it
-at::Tensor scratch(size_t bytes, const at::Tensor& like) {
-  return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(torch::kUInt8));
 }
 
 int launch_forward(const FaFwdParams& p, Differential* diff, const at::Tensor& q, int64_t num_heads) {
@@ -1039,6 +1023,7 @@ bool get_single_kernel_backward() { return (g_bwd_flags & FA_BWD_SINGLE_KERNEL) 
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_pages(m);
   m.def("fwd", &mha_fwd, "Forward pass", py::arg("q"), py::arg("k"), py::arg("v"), py::arg("softmax_scale"),
         py::arg("is_causal"), py::arg("out") = py::none(), py::arg("lse") = py::none(),
         py::arg("causal_shift") = py::none());

@@ -402,6 +402,59 @@ typedef struct FaDiffKvcacheParams {
 size_t fa_diff_kvcache_workspace_bytes(const FaDiffKvcacheParams* p);
 int fa_diff_kvcache(const FaDiffKvcacheParams* p, int32_t* verdict, int32_t token, fa_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------- */
+/* The pages of a paged KV cache (the one that fa_kvcache() reads): reserving, forking, freeing,   */
+/* compacting and copying them, on the device.  Tables: a row per sequence, whose pages come first  */
+/* and -1 behind them; page_refs[p]: how many rows hold page p, 0 = free.  Free pages are taken in    */
+/* ascending order.  No call synchronises; calls on the same tables have to be ordered (one stream).  */
+/* Scratch: fa_pages_workspace_bytes(rows, num_pages, entries) bytes, 256-byte aligned, not shared by   */
+/* calls that may overlap; entries: n of the call, or 0.  No counterpart in the reference.           */
+/* ------------------------------------------------------------------------------------------- */
+typedef struct FaPageTables {
+  int32_t* block_table;    /* (rows, columns), consecutive rows row_stride elements apart          */
+  int32_t* cache_seqlens;  /* (rows) tokens; fa_pages_compact() does not look at them               */
+  int32_t* page_refs;      /* (num_pages)                                                       */
+  int64_t row_stride;
+  int32_t rows, columns, num_pages;
+  int32_t reserved0;
+} FaPageTables;
+
+typedef struct FaPageCaches {
+  void* const* base;           /* host array: K and V of every layer, page 0                       */
+  const int64_t* page_stride;  /* host array: BYTES between consecutive pages of each              */
+  int64_t page_bytes;          /* a page, contiguous; a multiple of 16                            */
+  int32_t count;
+  int32_t reserved0;
+} FaPageCaches;
+
+size_t fa_pages_workspace_bytes(int32_t rows, int32_t num_pages, int32_t entries);
+
+/* Pages for cache_seqlens[r] + new_tokens[r] tokens (new_tokens NULL: new_tokens_all each; negative counts as 0).  Rows are   */
+/* served in order while the free pages last: a row is granted all it needs, or nothing; what a refused row needs counts       */
+/* against the rows behind it.  A row whose columns do not suffice is refused and counts for nothing.  granted[r]: 1 or 0.     */
+int fa_pages_reserve(const FaPageTables* t, const int32_t* new_tokens, int32_t new_tokens_all, int32_t page_size, uint8_t* granted,
+                     void* workspace, size_t workspace_bytes, fa_stream_t stream);
+
+/* Entry i makes row children[i], which holds no page, a copy of row parents[i]: the full pages of its tokens are shared, the    */
+/* tokens of a page that is not full are copied to a free page.  Entries are served in order; refused (granted[i] = 0): rows     */
+/* out of range (-1 for padding), a child that holds pages or that an earlier entry names, a parent that holds none or fewer     */
+/* than its length says, and entries for which no page is left.                                                        */
+int fa_pages_fork(const FaPageTables* t, const FaPageCaches* caches, const int32_t* parents, const int32_t* children, int32_t n,
+                  int32_t page_size, uint8_t* granted, void* workspace, size_t workspace_bytes, fa_stream_t stream);
+
+/* The rows give their pages back: entries -1, length 0.  Rows out of range are skipped, a row named twice is freed once.       */
+int fa_pages_free(const FaPageTables* t, const int32_t* rows, int32_t n, fa_stream_t stream);
+
+/* Moves pages so that those in use are the first *num_live (device memory), and rewrites the tables: the i-th page in use       */
+/* behind them goes to the i-th free one among them.                                                                 */
+int fa_pages_compact(const FaPageTables* t, const FaPageCaches* caches, int32_t* num_live, void* workspace, size_t workspace_bytes,
+                     fa_stream_t stream);
+
+/* Page dst[i] becomes a copy of page src[i] in every cache.  done[i] = 0, and nothing is copied: a page out of range, a         */
+/* destination that a later entry has too, a source that is the destination of another entry.                            */
+int fa_pages_copy(const FaPageCaches* caches, int32_t num_pages, const int32_t* src, const int32_t* dst, int32_t n, uint8_t* done,
+                  void* workspace, size_t workspace_bytes, fa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
