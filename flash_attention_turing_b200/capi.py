@@ -28,7 +28,6 @@ EXPORTED_SYMBOLS = (
     "fa_combine",
     "fa_combine_gather",
     "fa_sum_gather",
-    "fa_diff_fwd_workspace_bytes",
     "fa_diff_fwd",
     "fa_diff_bwd_workspace_bytes",
     "fa_diff_bwd",
@@ -98,7 +97,7 @@ class FaDiffWeights(C.Structure):
 
 
 class FaDiffFwdParams(C.Structure):
-    _fields_ = [("base", FaFwdParams), ("weights", FaDiffWeights), ("o2", _vp), *_strides("o2"), ("workspace", _vp), ("workspace_bytes", _sz)]
+    _fields_ = [("base", FaFwdParams), ("weights", FaDiffWeights), ("o2", _vp), *_strides("o2")]
 
 
 class FaDiffBwdParams(C.Structure):
@@ -176,11 +175,11 @@ def lib() -> C.CDLL:
         l.fa_bwd_workspace_bytes.argtypes = [C.POINTER(FaBwdParams)]
         l.fa_kvcache_workspace_bytes.restype = _sz
         l.fa_kvcache_workspace_bytes.argtypes = [C.POINTER(FaKvcacheParams)]
-        for name, struct in (("fa_diff_fwd", FaDiffFwdParams), ("fa_diff_bwd", FaDiffBwdParams), ("fa_diff_kvcache", FaDiffKvcacheParams)):
-            fn, size = getattr(l, name), getattr(l, name + "_workspace_bytes")
-            fn.restype, size.restype = C.c_int, _sz
-            fn.argtypes = [C.POINTER(struct), _vp, _i32, _vp] if name == "fa_diff_kvcache" else [C.POINTER(struct), _vp]
-            size.argtypes = [C.POINTER(struct)]
+        for fn, struct, more in ((l.fa_diff_fwd, FaDiffFwdParams, []), (l.fa_diff_bwd, FaDiffBwdParams, []),
+                                 (l.fa_diff_kvcache, FaDiffKvcacheParams, [_vp, _i32])):
+            fn.restype, fn.argtypes = C.c_int, [C.POINTER(struct), *more, _vp]
+        for fn, struct in ((l.fa_diff_bwd_workspace_bytes, FaDiffBwdParams), (l.fa_diff_kvcache_workspace_bytes, FaDiffKvcacheParams)):
+            fn.restype, fn.argtypes = _sz, [C.POINTER(struct)]
         tables, caches = C.POINTER(FaPageTables), C.POINTER(FaPageCaches)
         for name, args in (("reserve", [tables, _vp, _i32, _i32, _vp, _vp, _sz]), ("fork", [tables, caches, _vp, _vp, _i32, _i32, _vp, _vp, _sz]),
                            ("free", [tables, _vp, _i32]), ("compact", [tables, caches, _vp, _vp, _sz]),

@@ -6,7 +6,7 @@
 // come from the halves of the padded queries.
 #include <algorithm>
 
-#include "common.h"
+#include "diff.cuh"
 #include "fwd.h"
 #define FA_WAIT_INLINE
 #include "ptx.cuh"
@@ -17,11 +17,6 @@ namespace {
 constexpr int kThreads = 256;
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
-
-__device__ __forceinline__ float weight_of(const FaDiffWeights& w, int head) {
-  const int64_t at = w.count == 1 ? 0 : head * w.stride;
-  return w.is_half ? __half2float(static_cast<const __half*>(w.lam)[at]) : static_cast<const float*>(w.lam)[at];
-}
 
 // (batches, rows, heads, d) through strides; packed tensors are one batch
 struct View {
@@ -189,13 +184,6 @@ bool whole_units(std::initializer_list<int64_t> strides) {
   return true;
 }
 
-int check_weights(const FaDiffWeights& w, int h, const char* who) {
-  FA_CHECK_ARG(w.lam != nullptr, std::string(who) + ": lam must be non-NULL");
-  FA_CHECK_ARG(w.count == 1 || w.count == h, std::string(who) + ": weights.count must be 1 or h");
-  FA_CHECK_ARG(w.is_half == 0 || w.is_half == 1, std::string(who) + ": weights.is_half must be 0 or 1");
-  return FA_OK;
-}
-
 struct Rows {
   int64_t batches, rows;
   int64_t units(int h, int d) const { return batches * rows * h * (d / 8); }
@@ -225,15 +213,8 @@ int join(const JoinParams& jp, cudaStream_t stream) {
 }  // namespace
 }  // namespace fa
 
-extern "C" size_t fa_diff_fwd_workspace_bytes(const FaDiffFwdParams* p) {
+extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream) {
   using namespace fa;
-  if (p == nullptr || !plausible(p->base)) return 0;
-  return 2 * rows_of(p->base).map_bytes(p->base.h, p->base.d);
-}
-
-extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream_) {
-  using namespace fa;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   FA_CHECK_ARG(p != nullptr, "fa_diff_fwd: params is NULL");
   const FaFwdParams& b = p->base;
   FA_CHECK_ARG(b.q && b.k && b.v && b.o && b.lse, "fa_diff_fwd: q, k, v, o, lse must be non-NULL");
@@ -241,37 +222,9 @@ extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream_) {
   FA_CHECK_ARG(plausible(b), "fa_diff_fwd: bad b / h / h_k / seqlen_q");
   int rc = check_weights(p->weights, b.h, "fa_diff_fwd");
   if (rc != FA_OK) return rc;
-  FA_CHECK_ARG(aligned16(b.q) && aligned16(b.o) && aligned16(p->o2) &&
-                   whole_units({b.q_batch_stride, b.q_row_stride, b.q_head_stride, b.o_batch_stride, b.o_row_stride, b.o_head_stride,
-                                p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride}),
-               "fa_diff_fwd: q, o and o2 must be 16-byte aligned with strides that are multiples of 8 elements");
-  const Rows r = rows_of(b);
-  const size_t map_bytes = r.map_bytes(b.h, b.d);
-  if (p->workspace == nullptr || p->workspace_bytes < 2 * map_bytes)
-    return set_error(FA_ERR_WORKSPACE, "fa_diff_fwd: workspace smaller than fa_diff_fwd_workspace_bytes()");
-  FA_CHECK_ARG((reinterpret_cast<uintptr_t>(p->workspace) & 255) == 0, "fa_diff_fwd: workspace must be 256-byte aligned");
-  rc = check_device_sm100();
-  if (rc != FA_OK) return rc;
-  const int unit_bits = b.d == 128 ? 4 : 3;
-  __half* q_maps = static_cast<__half*>(p->workspace);
-  __half* o_maps = reinterpret_cast<__half*>(static_cast<uint8_t*>(p->workspace) + map_bytes);
-  SplitParams sp = {};
-  sp.q = view(b.q, b.q_batch_stride, b.q_row_stride, b.q_head_stride);
-  sp.q_maps = q_maps;
-  sp.units = r.units(b.h, b.d);
-  sp.rows = static_cast<int>(r.rows), sp.h = b.h, sp.unit_bits = unit_bits;
-  rc = split(sp, stream);
-  if (rc != FA_OK) return rc;
-  FaFwdParams f = b;
-  f.q = q_maps, f.o = o_maps, f.h = 2 * b.h;
-  f.q_head_stride = f.o_head_stride = b.d;
-  f.q_row_stride = f.o_row_stride = static_cast<int64_t>(2) * b.h * b.d;
-  f.q_batch_stride = f.o_batch_stride = f.q_row_stride * r.rows;
-  rc = fa_fwd(&f, stream);
-  if (rc != FA_OK) return rc;
-  return join(JoinParams{o_maps, view(b.o, b.o_batch_stride, b.o_row_stride, b.o_head_stride),
-                         view(p->o2, p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride), p->weights, sp.units, sp.rows, b.h, unit_bits},
-              stream);
+  FA_CHECK_ARG(aligned16(p->o2) && whole_units({p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride}),
+               "fa_diff_fwd: o2 must be 16-byte aligned with strides that are multiples of 8 elements");
+  return run_fwd(&b, 0, static_cast<cudaStream_t>(stream), false, false, p);
 }
 
 extern "C" size_t fa_diff_bwd_workspace_bytes(const FaDiffBwdParams* p) {

@@ -7,8 +7,9 @@ namespace fa {
 
 // Same as fa_fwd(); seqused_k_add is added to every seqused_k[b] on the device.  overlap: the previous kernel of the stream
 // lets this one start early (launch_overlapped).  checked: the host refuses lengths beyond the capacity; they are neither read nor
-// reported.
-int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap = false, bool checked = false);
+// reported.  diff: differential attention, with p = &diff->base.
+int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap = false, bool checked = false,
+            const FaDiffFwdParams* diff = nullptr);
 
 #ifdef __CUDACC__
 // What a sequence of a cache holds, limited to what it can hold; in 64 bits, a length may be any int32.  Beyond the capacity:

@@ -28,6 +28,7 @@
 // Replaces flash_fwd_kernel / compute_attn_1rowblock of the reference
 // (csrc/flash_attn/src/flash_fwd_kernel.h:23-664) including its masking (src/mask.h:20-69), its
 // varlen offsets (src/block_info.h:3-36) and its launch grid (src/flash_fwd_launch_template.h:60-75).
+#include "diff.cuh"
 #include "fwd.h"
 
 #include "packed_rows.cuh"
@@ -54,6 +55,11 @@ constexpr int kSchedReaders = kTiles * kSoftmaxWarpsPerTile + 2;  // softmax war
 // B16 S1024, 1728 us at B2 S16384 H16 D64; 4 with the hand-over pinned: 2213 / 215 / 1653; 6 pinned: 2192 / 212 / 1602.
 constexpr int kPvFirst = 6;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+// Differential attention: every fourth pair of exponentials is a polynomial, on the FMA pipes beside the special-function unit, which
+// 16 exponentials a clock and SM keep busy for 1024 clocks a tile.  D = 64, where the products take half of that: S16384 H18 without mask
+// 3610 -> 3250 us, B2 S4096 H16 causal 1.07 -> 0.97 of two plain query heads' time; every third the same, every second 3390.  D = 128
+// runs at the power cap (1.65 GHz) and does not care: B1 S8192 Hq16 Hkv4 causal 402 us with and without.
+constexpr int kPolynomialEvery = 4;
 
 struct FwdKernelParams {
   CUtensorMap tm_q;
@@ -86,6 +92,10 @@ struct FwdKernelParams {
   int b;              // sequences
   int section_rows;   // see section_item()
   int group;          // query heads per key head
+  // differential attention
+  FaDiffWeights weights;
+  __half* o2;         // A_2 V, or null
+  int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
 };
 
 template <int D>
@@ -110,7 +120,9 @@ struct __align__(16) Work {
   int row0, sk, shift, sq;
   int batch, head, head_k, q_off;
   int k_off, bq, bk, nkb;
-  int fix_v_tail, pad[3];
+  int fix_v_tail;
+  float lam;  // differential: the weight of the head
+  int pad[2];
 };
 
 struct Barriers {
@@ -129,6 +141,8 @@ struct Barriers {
   uint64_t sched_full[kSchedDepth];
   uint64_t sched_empty[kSchedDepth];
   uint64_t sched_go;        // the current item is two blocks from its end: time to claim the next one
+  uint64_t factors[4];      // differential: both maps' factors of a warp's 32 rows are in shared memory
+  uint64_t o_read;          // differential: O of both maps has been read, the next item's products may overwrite it
   Work items[kSchedDepth];
   uint32_t tmem_base;
   int abort_flag;
@@ -139,7 +153,7 @@ static_assert(sizeof(Barriers) <= 1024, "barrier block");
 // cannot be scheduled at all
 static_assert((kNumThreads / 32 + 3) / 4 * 32 * 168 <= 16384, "register file of one SM sub-partition");
 
-template <int D, int kItemRows>
+template <int D, int kItemRows, bool kDiff>
 __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, int head, int mpair, Work& w) {
   w.mpair = mpair;
   w.batch = batch;
@@ -160,12 +174,12 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
   w.head_k = w.head / (D == 64 ? p.h / p.h_k : p.group);
   // causal diagonal: key j is visible to query i iff j <= i + shift
   w.shift = (p.is_causal == 2) ? p.causal_shift : w.sk - w.sq;
-  if (kItemRows == kBlockM) w.sq = min(w.sq, w.row0 + kBlockM);  // the rows after the item's only tile are not its own
+  if (kItemRows == kBlockM && !kDiff) w.sq = min(w.sq, w.row0 + kBlockM);  // the rows after the item's only tile are not its own
   // number of K/V blocks each tile visits
   w.nkb = (w.sk + kBlockN - 1) / kBlockN;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
-    const int r0 = w.row0 + t * kBlockM;
+    const int r0 = w.row0 + (kDiff ? 0 : t * kBlockM);
     int n = w.nkb;
     if (p.is_causal) {
       const int x = r0 + kBlockM + w.shift;  // one past the last visible key of the tile's last row
@@ -179,12 +193,22 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
   // from a packed tensor or a cache (the next sequence, or never-written cache rows).  Their scores are
   // masked, but P = 0 times a NaN/Inf bit pattern in V would still poison O, so those V rows are zeroed
   // in shared memory before the last PV MMA.  (Dense tensors: TMA fills out-of-range rows with zeros.)
+  if constexpr (kDiff) w.lam = weight_of(p.weights, head);
   w.fix_v_tail = (p.seqused_k != nullptr || varlen_k) && (w.sk % kBlockN) != 0 && w.nb_max == w.nkb && w.nkb > 0;
 }
 
 // kItemRows = 256: two Q tiles per item.  kItemRows = 128: one, the second tile's warps have nothing to do (dense batches, chosen
 // in launch_fwd).
-template <int D, int kItemRows>
+//
+// kDiff: differential attention, O = O_0 / l_0 - lam O_1 / l_1.  The two tiles of an item are the two maps of the same 128 rows: Q and
+// K tiles hold both halves of the head dimension, tile t multiplies the D / 32 slices of its half, and V is shared, so that the loads, the
+// barriers and the softmax are those of two tiles at 3/4 of their products.  At the end a warp needs the other map's factor of its
+// rows (through shared memory) and its accumulator (the same TMEM lanes), and each of the two stores half of the columns: the maps are
+// subtracted in 32 bits, and their outputs are neither rounded nor written by themselves.
+// B1 S8192 Hq16 Hkv4 D128 causal 402 us (684 TFLOP/s of 4 h d a pair; 6 are executed), where two query heads with half of d set to zero
+// take 448 and the kernels that lay them out and subtract 60 more; 37 heads S4096 without mask 462 : 518; S1024 and shorter about the
+// same by itself.
+template <int D, int kItemRows, bool kDiff>
 __global__ void __maxnreg__(168)
 fwd_kernel(const __grid_constant__ FwdKernelParams p) {
   using C = Cfg<D>;
@@ -202,6 +226,8 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
   uint8_t* sK = sQ + kTiles * C::kTileBytes;
   uint8_t* sV = sK + C::kStages * C::kTileBytes;
   Barriers* bars = reinterpret_cast<Barriers*>(sV + C::kStages * C::kTileBytes);
+  static_assert(!kDiff || kItemRows == kBlockM, "differential: an item is 128 rows");
+  float* factors = reinterpret_cast<float*>(sQ + C::kTileBytes);  // differential: [item & 1][map][row], where the second Q tile would be
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -230,6 +256,10 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       mbar_init(&bars->sched_empty[s], kSchedReaders);
     }
     mbar_init(&bars->sched_go, 1);
+    if constexpr (kDiff) {
+      for (int i = 0; i < 4; ++i) mbar_init(&bars->factors[i], 2);
+      mbar_init(&bars->o_read, kTiles * kSoftmaxWarpsPerTile);
+    }
     bars->abort_flag = 0;
     fence_mbar_init();
     grid_dependency_wait();  // a cache append, or the kernel that clears the unused rows
@@ -286,8 +316,9 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
             // which are at least h * ceil(length / 256) and at most h more -- so an index maps to a live item
             // except for at most one slot per (sequence, head), whatever the spread of the lengths.  The indices
             // a CTA claims only grow, so the sequence is found by walking forward from the last one.
-            while (seq + 1 < p.b && p.h * ((p.cu_seqlens_q[seq + 1] >> 8) + seq + 1) <= next) ++seq;
-            const int v0 = (p.cu_seqlens_q[seq] >> 8) + seq, v1 = (p.cu_seqlens_q[seq + 1] >> 8) + seq + 1;
+            constexpr int kShift = kDiff ? 7 : 8;  // 128 or 256 rows
+            while (seq + 1 < p.b && p.h * ((p.cu_seqlens_q[seq + 1] >> kShift) + seq + 1) <= next) ++seq;
+            const int v0 = (p.cu_seqlens_q[seq] >> kShift) + seq, v1 = (p.cu_seqlens_q[seq + 1] >> kShift) + seq + 1;
             const int rel = next - p.h * v0, cnt = v1 - v0;
             const int len = p.cu_seqlens_q[seq + 1] - p.cu_seqlens_q[seq];
             batch = seq, head = 0, mpair = -1;
@@ -295,12 +326,13 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
               const int keys = p.cu_seqlens_k ? p.cu_seqlens_k[seq + 1] - p.cu_seqlens_k[seq] : p.seqlen_k;
               const HeadPlace at = section_item(rel, p.h, cnt, p.group, keys, p.section_rows);
               head = at.head;
-              mpair = (len + kTiles * kBlockM - 1) / (kTiles * kBlockM) - 1 - at.place;  // < 0: the spare slot
+              constexpr int kRows = kDiff ? kBlockM : kTiles * kBlockM;
+              mpair = (len + kRows - 1) / kRows - 1 - at.place;  // < 0: the spare slot
             }
           }
           const int sq = p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q;
           if (mpair >= 0 && mpair * kItemRows < sq) {
-            make_work<D, kItemRows>(p, batch, head, mpair, it);
+            make_work<D, kItemRows, kDiff>(p, batch, head, mpair, it);
             if (p.seqused_k && p.status && head == 0 && mpair == 0 &&
                 cache_length(p.seqused_k[batch], p.seqused_k_add, p.k_capacity, p.checked).report)
               atomicOr(p.status, kStatusCapacityClamped);
@@ -343,10 +375,10 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       if (lane == 0) {
         ok = mbar_wait(&bars->q_empty, (nq & 1) ^ 1, ctx);
         if (ok) {
-          const int ntl = (w.nb[0] > 0) + (w.nb[1] > 0);
+          const int ntl = kDiff ? 1 : (w.nb[0] > 0) + (w.nb[1] > 0);
           mbar_arrive_expect_tx(&bars->q_full, ntl * C::kTileBytes);
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
+          for (int t = 0; t < (kDiff ? 1 : kTiles); ++t) {
             if (w.nb[t] > 0) {
 #pragma unroll
               for (int c = 0; c < C::kChunks; ++c)
@@ -418,12 +450,13 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       // S_t = Q_t K^T with K in ring stage s: D/16 MMAs of K=16; slice k lives in swizzle chunk k/4 at byte
       // (k%4)*32.
       auto issue_qk = [&](int t, int s) {
-        const uint64_t qd = make_smem_desc(sQ_addr + t * C::kTileBytes, 16, 1024);
+        const uint64_t qd = make_smem_desc(sQ_addr + (kDiff ? 0 : t * C::kTileBytes), 16, 1024);
         const uint64_t kd = make_smem_desc(sK_addr + s * C::kTileBytes, 16, 1024);
         const uint32_t d_addr = tmem_base + C::kColS + t * 128;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * C::kChunkBytes + (k & 3) * 32;
+        for (int k = 0; k < (kDiff ? D / 32 : D / 16); ++k) {
+          const int slice = kDiff ? t * (D / 32) + k : k;  // differential: tile t has the slices of its half
+          const uint32_t off = (slice >> 2) * C::kChunkBytes + (slice & 3) * 32;
           mma_ss(d_addr, desc_advance(qd, off), desc_advance(kd, off), idesc_qk, k > 0);
         }
       };
@@ -474,6 +507,8 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
             if (has_pv) {
               const uint32_t par = (cs_par >> t) & 1;
               if (!(ok = mbar_wait_hot(&bars->p_full[t][0], par, ctx))) break;
+              // both O of the item before are read by warps of both tiles
+              if (kDiff && t == 0 && j == 0 && nq > 0 && !(ok = mbar_wait(&bars->o_read, (nq - 1) & 1, ctx))) break;
               tc_fence_after_sync();
               issue_pv(t, s, 0, j == 0);
               if (!(ok = mbar_wait_hot(&bars->p_full[t][1], par, ctx))) break;
@@ -536,7 +571,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       const volatile Work& w = bars->items[n % kSchedDepth];
       if (w.mpair < 0) break;
-      const int nbt = w.nb[t], sk = w.sk, shift = w.shift, row = w.row0 + t * kBlockM + row_in_tile, nb_max = w.nb_max;
+      const int nbt = w.nb[t], sk = w.sk, shift = w.shift, row = w.row0 + (kDiff ? 0 : t * kBlockM) + row_in_tile, nb_max = w.nb_max;
 
       float m = -INFINITY;  // lazily updated reference maximum of the row (raw score units)
       float l = 0.f;        // row sum relative to m
@@ -632,7 +667,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 x = ffma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, nm2);
-            const float2 e = make_float2(ex2f(x.x), ex2f(x.y));
+            const float2 e = kDiff && i % kPolynomialEvery == kPolynomialEvery - 1 ? exp2_polynomial(x) : make_float2(ex2f(x.x), ex2f(x.y));
             sum[i & 3] = fadd2(sum[i & 3], e);  // independent chains, as for the maximum
             pk[i] = pack_half2(e.x, e.y);
           }
@@ -669,6 +704,80 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
                   w.head * p.o_head_stride;
       }
       __half* orow = p.o + o_index;
+      if constexpr (kDiff) {
+        // this warp's factor to the other map's warp of the same rows, and half of the columns of both maps' rows
+        float inv = 0.f, lse_val = 0.f;
+        if (nbt > 0 && l > 0.f && m != -INFINITY) {
+          inv = 1.f / l;
+          lse_val = (m * c + __log2f(l)) * kLn2;
+        }
+        if (row_valid) p.lse[(static_cast<int64_t>(w.batch) * 2 * p.h + 2 * w.head + t) * p.lse_row_stride + row] = lse_val;
+        const int col0 = t * (D / 2);
+        __half* o2row = nullptr;
+        if (p.o2 != nullptr)
+          o2row = p.o2 + (varlen_q ? static_cast<int64_t>(w.q_off + row) * p.o2_row_stride
+                                   : w.batch * p.o2_batch_stride + static_cast<int64_t>(row) * p.o2_row_stride) + w.head * p.o2_head_stride;
+        auto store = [&](__half* to, const uint32_t (&x)[32], int col) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 v;
+            v.x = pack_half2(__uint_as_float(x[8 * i + 0]), __uint_as_float(x[8 * i + 1]));
+            v.y = pack_half2(__uint_as_float(x[8 * i + 2]), __uint_as_float(x[8 * i + 3]));
+            v.z = pack_half2(__uint_as_float(x[8 * i + 4]), __uint_as_float(x[8 * i + 5]));
+            v.w = pack_half2(__uint_as_float(x[8 * i + 6]), __uint_as_float(x[8 * i + 7]));
+            *reinterpret_cast<uint4*>(to + col + i * 8) = v;
+          }
+        };
+        if (nbt > 0) {
+          float* mine = factors + (no & 1) * 2 * kBlockM + row_in_tile;
+          mine[t * kBlockM] = inv;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->factors[quarter]);
+          if (!(ok = mbar_wait_warp(&bars->o_full[0], no & 1, ctx))) break;
+          if (!(ok = mbar_wait_warp(&bars->o_full[1], no & 1, ctx))) break;
+          if (!(ok = mbar_wait_warp(&bars->factors[quarter], no & 1, ctx))) break;
+          tc_fence_after_sync();
+          // a row without a visible key has no factor, and its sums may hold what hidden values are
+          const float other = mine[(t ^ 1) * kBlockM], inv1 = t == 0 ? inv : other, inv2 = t == 0 ? other : inv;
+          const float minus = -w.lam * inv2;
+          const uint32_t tO1 = tmem_base + lane_base + C::kColO + col0, tO2 = tO1 + D;
+#pragma unroll 1
+          for (int q = 0; q < D / 64; ++q) {
+            uint32_t a[32], b[32];
+            tmem_ld32(tO1 + q * 32, a);
+            tmem_ld32(tO2 + q * 32, b);
+            tmem_wait_ld();
+            if (q == D / 64 - 1) {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars->o_read);
+            }
+            if (row_valid) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                a[i] = inv1 == 0.f ? 0u : __float_as_uint(fmaf(__uint_as_float(b[i]), minus, __uint_as_float(a[i]) * inv1));
+              store(orow, a, col0 + q * 32);
+              if (o2row != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) b[i] = inv2 == 0.f ? 0u : __float_as_uint(__uint_as_float(b[i]) * inv2);
+                store(o2row, b, col0 + q * 32);
+              }
+            }
+          }
+          ++no;
+        } else if (row_valid) {  // no key block is visible to any row of this tile
+          const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            *reinterpret_cast<uint4*>(orow + col0 + i * 8) = z;
+            if (o2row != nullptr) *reinterpret_cast<uint4*>(o2row + col0 + i * 8) = z;
+          }
+        }
+        g += nb_max;
+        __syncwarp();
+        if (lane == 0) release_item(n);
+        continue;
+      }
       if (nbt > 0) {
         if (!(ok = mbar_wait_warp(&bars->o_full[t], no & 1, ctx))) break;
         ++no;
@@ -757,14 +866,14 @@ __global__ void __launch_bounds__(kClearThreads) clear_unused_rows_kernel(const 
   }
 }
 
-template <int D, int kItemRows>
+template <int D, int kItemRows, bool kDiff>
 int launch_items(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_q, bool overlap, cudaStream_t stream) {
   using C = Cfg<D>;
   static bool configured[64] = {};
   int dev = 0;
   FA_CHECK_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    FA_CHECK_CUDA(cudaFuncSetAttribute(fwd_kernel<D, kItemRows>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    FA_CHECK_CUDA(cudaFuncSetAttribute(fwd_kernel<D, kItemRows, kDiff>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        C::kSmemBytes));
     configured[dev & 63] = true;
   }
@@ -773,7 +882,7 @@ int launch_items(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_
   if (sms <= 0 || kp.sched == nullptr) return set_error(FA_ERR_CUDA, "fa_fwd: device attributes not available");
   kp.items_x = (seqlen_q + kItemRows - 1) / kItemRows;
   kp.b = b;
-  const int64_t total = kp.cu_seqlens_q ? static_cast<int64_t>(h) * (total_q / (kTiles * kBlockM) + b)
+  const int64_t total = kp.cu_seqlens_q ? static_cast<int64_t>(h) * (total_q / (kDiff ? kBlockM : kTiles * kBlockM) + b)
                                         : static_cast<int64_t>(kp.items_x) * h * b;
   FA_CHECK_ARG(total < (1ll << 30), "fa_fwd: too many work items");
   kp.total_items = static_cast<int>(total);
@@ -781,9 +890,9 @@ int launch_items(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_
   kp.section_rows = total <= sms ? 0 : section_rows(kp.is_causal != 0, seqlen_q, kp.seqused_k ? kp.k_capacity : kp.seqlen_k, 4 * D);
   const int grid = kp.total_items < sms ? kp.total_items : sms;  // one CTA per SM (202 KB of shared memory each)
   if (overlap) {
-    FA_CHECK_CUDA(launch_overlapped(fwd_kernel<D, kItemRows>, dim3(grid), kNumThreads, C::kSmemBytes, stream, kp));
+    FA_CHECK_CUDA(launch_overlapped(fwd_kernel<D, kItemRows, kDiff>, dim3(grid), kNumThreads, C::kSmemBytes, stream, kp));
   } else {
-    fwd_kernel<D, kItemRows><<<grid, kNumThreads, C::kSmemBytes, stream>>>(kp);
+    fwd_kernel<D, kItemRows, kDiff><<<grid, kNumThreads, C::kSmemBytes, stream>>>(kp);
     FA_CHECK_CUDA(cudaGetLastError());
   }
   return FA_OK;
@@ -793,11 +902,12 @@ int launch_items(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_
 // than the chip has SMs gets an SM for every tile instead: B2 S512 H8 D64 15.1 -> 13.6 us, B1 S1000 H16 D128 causal 24.8 -> 21.8, B1 S2304
 // H8 D128 43.8 -> 38.1; with more tiles than SMs some SMs would run two items in turn, which takes longer than a pair.
 template <int D>
-int launch_fwd(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_q, bool overlap, cudaStream_t stream) {
+int launch_fwd(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_q, bool diff, bool overlap, cudaStream_t stream) {
+  if (diff) return launch_items<D, kBlockM, true>(kp, b, h, seqlen_q, total_q, overlap, stream);
   const int64_t tiles = static_cast<int64_t>((seqlen_q + kBlockM - 1) / kBlockM) * h * b;
   if (kp.cu_seqlens_q == nullptr && tiles <= device_sm_count())
-    return launch_items<D, kBlockM>(kp, b, h, seqlen_q, total_q, overlap, stream);
-  return launch_items<D, kTiles * kBlockM>(kp, b, h, seqlen_q, total_q, overlap, stream);
+    return launch_items<D, kBlockM, false>(kp, b, h, seqlen_q, total_q, overlap, stream);
+  return launch_items<D, kTiles * kBlockM, false>(kp, b, h, seqlen_q, total_q, overlap, stream);
 }
 
 }  // namespace
@@ -805,7 +915,7 @@ int launch_fwd(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_q,
 
 namespace fa {
 
-int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap, bool checked) {
+int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap, bool checked, const FaDiffFwdParams* diff) {
   FA_CHECK_ARG(p != nullptr, "fa_fwd: params is NULL");
   FA_CHECK_ARG(p->q && p->k && p->v && p->o && p->lse, "fa_fwd: q, k, v, o, lse must be non-NULL");
   if (p->d != 64 && p->d != 128)
@@ -886,19 +996,25 @@ int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool o
   kp.block_table_batch_stride = p->block_table_batch_stride;
   kp.page_size = p->page_size;
   kp.group = p->h / p->h_k;
+  kp.weights = diff ? diff->weights : FaDiffWeights{};
+  kp.o2 = diff ? static_cast<__half*>(diff->o2) : nullptr;
+  kp.o2_batch_stride = diff ? diff->o2_batch_stride : 0;
+  kp.o2_row_stride = diff ? diff->o2_row_stride : 0;
+  kp.o2_head_stride = diff ? diff->o2_head_stride : 0;
   kp.status = device_status_ptr();
   if (p->flags == FA_FWD_ZERO_UNUSED_ROWS && varlen_q) {  // no other value: see the header
     const PackedRows rows{kp.o, kp.o_row_stride, kp.o_head_stride, p->total_q, p->h, p->d, p->cu_seqlens_q, p->b};
+    const int lse_heads = diff ? 2 * p->h : p->h;  // rows of A_2 V outside every sequence are read by no one
     const int sms = device_sm_count();
     if (sms <= 0) return set_error(FA_ERR_CUDA, "fa_fwd: device attributes not available");
-    const UnusedLse lse{p->lse, p->lse_row_stride, p->b, p->h, p->seqlen_q};
+    const UnusedLse lse{p->lse, p->lse_row_stride, p->b, lse_heads, p->seqlen_q};
     clear_unused_rows_kernel<<<sms, kClearThreads, 0, stream>>>(rows, lse, kp.status);
     FA_CHECK_CUDA(cudaGetLastError());
     overlap = true;
   }
 
-  if (p->d == 128) return launch_fwd<128>(kp, p->b, p->h, p->seqlen_q, p->total_q, overlap, stream);
-  return launch_fwd<64>(kp, p->b, p->h, p->seqlen_q, p->total_q, overlap, stream);
+  if (p->d == 128) return launch_fwd<128>(kp, p->b, p->h, p->seqlen_q, p->total_q, diff != nullptr, overlap, stream);
+  return launch_fwd<64>(kp, p->b, p->h, p->seqlen_q, p->total_q, diff != nullptr, overlap, stream);
 }
 
 }  // namespace fa

@@ -526,6 +526,22 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// 2^x without the special-function unit, for x up to 127: x = n + f with n the nearest integer, a polynomial of degree 4 in f (its
+// coefficients minimise the largest relative error over [-1/2, 1/2], 2.7e-6), and n added to the exponent.  Below -125 (masked scores
+// are -inf): 2^-125, far below what fp16 and the row sums hold.  NaN stays NaN or becomes infinite.
+__device__ __forceinline__ float2 exp2_polynomial(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x.x));  // -125
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are the integer
+  const float2 t = fadd2(x, magic), f = fsub2(x, fsub2(t, magic));
+  float2 p = ffma2(make_float2(0.009570102207362652f, 0.009570102207362652f), f, make_float2(0.05591786280274391f, 0.05591786280274391f));
+  p = ffma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = ffma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = ffma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

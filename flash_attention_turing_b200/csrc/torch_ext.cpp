@@ -77,9 +77,6 @@ int launch_forward(const FaFwdParams& p, Differential* diff, const at::Tensor& q
     d.o2 = o2.data_ptr();
     d.o2_batch_stride = batch ? o2.stride(0) : 0, d.o2_row_stride = o2.stride(batch), d.o2_head_stride = o2.stride(batch + 1);
   }
-  at::Tensor workspace = scratch(fa_diff_fwd_workspace_bytes(&d), q);
-  d.workspace = workspace.data_ptr();
-  d.workspace_bytes = workspace.numel();
   return fa_diff_fwd(&d, current_stream());
 }
 

@@ -371,11 +371,8 @@ typedef struct FaDiffFwdParams {
   FaDiffWeights weights;
   void* o2;           /* NULL, or A_2 V (fp16, the shape of o, its own strides): fa_diff_bwd() needs it */
   int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
-  void* workspace;    /* 256-byte aligned, fa_diff_fwd_workspace_bytes() bytes                    */
-  size_t workspace_bytes;
 } FaDiffFwdParams;
 
-size_t fa_diff_fwd_workspace_bytes(const FaDiffFwdParams* p);
 int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream);
 
 /* Backward: dq, dk, dv (per KV head, summed over its query heads) and the gradient of the weights. */
