@@ -71,9 +71,18 @@ int make_tensor_map_4d(CUtensorMap* map, const void* base, int d, int64_t heads,
                         static_cast<cuuint64_t>(batch_stride) * 2};
   cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(box_rows), 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult res = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), gdim, gstr,
-                        box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto run = [&] {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), gdim, gstr,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult res = run();
+  if (res == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread that has made no runtime call yet has no context
+    int dev = 0;
+    FA_CHECK_CUDA(cudaGetDevice(&dev));
+    FA_CHECK_CUDA(cudaSetDevice(dev));
+    res = run();
+  }
   if (res != CUDA_SUCCESS)
     return set_error(FA_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed with code " +
                                       std::to_string(static_cast<int>(res)));

@@ -107,71 +107,6 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   }
 }
 
-// dQ: each half from the query head of its map
-__global__ void __launch_bounds__(kThreads) gather_dq_kernel(const __half* dq_maps, const View dq, int64_t total, int rows, int h, int unit_bits) {
-  const int units = 1 << unit_bits;
-  for (int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; idx < total; idx += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const Place at = place_of(idx, rows, h, unit_bits);
-    const int64_t from = ((idx >> unit_bits) * 2 << unit_bits) + at.unit;
-    *dq.at(at.batch, at.row, at.head, at.unit) = reinterpret_cast<const uint4*>(dq_maps)[from + (2 * at.unit < units ? 0 : units)];
-  }
-}
-
-// dlam_h = -sum over rows of dO . (A_2 V): partial sums of chunks of rows, then their sum, each in a fixed order
-constexpr int kLamChunks = 64;
-struct LamParams {
-  View o2, dout;
-  float* partial;  // (h, kLamChunks)
-  void* dlam;
-  int64_t rows;    // batches * rows of a batch
-  int rows_of_batch, h, unit_bits, is_half, one;
-  const int* cu_seqlens;  // packed: rows outside [cu[0], cu[b]) do not count
-  int b;
-};
-__device__ __forceinline__ float block_sum(float x, float* shared) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0.f;
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) x += shared[i];
-  return x;
-}
-__global__ void __launch_bounds__(kThreads) lam_partial_kernel(const __grid_constant__ LamParams p) {
-  __shared__ float shared[kThreads / 32];
-  const int head = blockIdx.x, chunk = blockIdx.y;
-  int64_t first = 0, last = p.rows;
-  if (p.cu_seqlens != nullptr) first = max(p.cu_seqlens[0], 0), last = min(static_cast<int64_t>(p.cu_seqlens[p.b]), p.rows);
-  const int64_t n = max(last - first, static_cast<int64_t>(0));
-  const int64_t begin = first + n * chunk / kLamChunks, end = first + n * (chunk + 1) / kLamChunks;
-  const int units = 1 << p.unit_bits, unit = threadIdx.x & (units - 1);
-  float sum = 0.f;
-  for (int64_t r = begin + (threadIdx.x >> p.unit_bits); r < end; r += kThreads >> p.unit_bits) {
-    const int64_t batch = r / p.rows_of_batch, row = r - batch * p.rows_of_batch;
-    const uint4 a = *p.o2.at(batch, row, head, unit), b = *p.dout.at(batch, row, head, unit);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = __half22float2(reinterpret_cast<const __half2*>(&a)[i]), y = __half22float2(reinterpret_cast<const __half2*>(&b)[i]);
-      sum = fmaf(x.x, y.x, sum);
-      sum = fmaf(x.y, y.y, sum);
-    }
-  }
-  sum = block_sum(sum, shared);
-  if (threadIdx.x == 0) p.partial[head * kLamChunks + chunk] = sum;
-}
-__global__ void __launch_bounds__(kThreads) lam_sum_kernel(const __grid_constant__ LamParams p) {
-  __shared__ float shared[kThreads / 32];
-  const int n = p.one ? p.h * kLamChunks : kLamChunks;
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < n; i += kThreads) sum += p.partial[blockIdx.x * kLamChunks + i];
-  sum = block_sum(sum, shared);
-  if (threadIdx.x != 0) return;
-  if (p.is_half) static_cast<__half*>(p.dlam)[blockIdx.x] = __float2half_rn(-sum);
-  else static_cast<float*>(p.dlam)[blockIdx.x] = -sum;
-}
-
 View view(const void* base, int64_t batch_stride, int64_t row_stride, int64_t head_stride) {
   return View{static_cast<__half*>(const_cast<void*>(base)), batch_stride, row_stride, head_stride};
 }
@@ -225,75 +160,6 @@ extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream) {
   FA_CHECK_ARG(aligned16(p->o2) && whole_units({p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride}),
                "fa_diff_fwd: o2 must be 16-byte aligned with strides that are multiples of 8 elements");
   return run_fwd(&b, 0, static_cast<cudaStream_t>(stream), false, false, p);
-}
-
-extern "C" size_t fa_diff_bwd_workspace_bytes(const FaDiffBwdParams* p) {
-  using namespace fa;
-  if (p == nullptr || !plausible(p->base)) return 0;
-  FaBwdParams f = p->base;
-  f.h *= 2, f.flags &= FA_BWD_ZERO_UNUSED_ROWS;
-  return 4 * rows_of(p->base).map_bytes(p->base.h, p->base.d) + align256(static_cast<size_t>(p->base.h) * kLamChunks * 4) + fa_bwd_workspace_bytes(&f);
-}
-
-extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
-  using namespace fa;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  FA_CHECK_ARG(p != nullptr, "fa_diff_bwd: params is NULL");
-  const FaBwdParams& b = p->base;
-  FA_CHECK_ARG(b.q && b.k && b.v && b.o && p->o2 && b.dout && b.lse && b.dq && b.dk && b.dv && p->dlam,
-               "fa_diff_bwd: q, k, v, o, o2, dout, lse, dq, dk, dv, dlam must be non-NULL");
-  if (b.d != 64 && b.d != 128) return set_error(FA_ERR_UNSUPPORTED, "fa_diff_bwd: head_dim must be 64 or 128");
-  FA_CHECK_ARG(plausible(b), "fa_diff_bwd: bad b / h / h_k / seqlen_q");
-  FA_CHECK_ARG((b.flags & ~FA_BWD_ZERO_UNUSED_ROWS) == 0, "fa_diff_bwd: flags must be 0 or FA_BWD_ZERO_UNUSED_ROWS");
-  int rc = check_weights(p->weights, b.h, "fa_diff_bwd");
-  if (rc != FA_OK) return rc;
-  FA_CHECK_ARG(aligned16(b.q) && aligned16(b.o) && aligned16(p->o2) && aligned16(b.dout) && aligned16(b.dq) &&
-                   whole_units({b.q_batch_stride, b.q_row_stride, b.q_head_stride, b.o_batch_stride, b.o_row_stride, b.o_head_stride,
-                                p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride, b.do_batch_stride, b.do_row_stride,
-                                b.do_head_stride, b.dq_batch_stride, b.dq_row_stride, b.dq_head_stride}),
-               "fa_diff_bwd: q, o, o2, dout and dq must be 16-byte aligned with strides that are multiples of 8 elements");
-  if (b.workspace == nullptr || b.workspace_bytes < fa_diff_bwd_workspace_bytes(p))
-    return set_error(FA_ERR_WORKSPACE, "fa_diff_bwd: workspace smaller than fa_diff_bwd_workspace_bytes()");
-  FA_CHECK_ARG((reinterpret_cast<uintptr_t>(b.workspace) & 255) == 0, "fa_diff_bwd: workspace must be 256-byte aligned");
-  rc = check_device_sm100();
-  if (rc != FA_OK) return rc;
-  const Rows r = rows_of(b);
-  const size_t map_bytes = r.map_bytes(b.h, b.d);
-  const int unit_bits = b.d == 128 ? 4 : 3;
-  uint8_t* ws = static_cast<uint8_t*>(b.workspace);
-  SplitParams sp = {};
-  sp.q = view(b.q, b.q_batch_stride, b.q_row_stride, b.q_head_stride);
-  sp.o = view(b.o, b.o_batch_stride, b.o_row_stride, b.o_head_stride);
-  sp.o2 = view(p->o2, p->o2_batch_stride, p->o2_row_stride, p->o2_head_stride);
-  sp.dout = view(b.dout, b.do_batch_stride, b.do_row_stride, b.do_head_stride);
-  sp.q_maps = reinterpret_cast<__half*>(ws), sp.o_maps = reinterpret_cast<__half*>(ws + map_bytes);
-  sp.do_maps = reinterpret_cast<__half*>(ws + 2 * map_bytes);
-  __half* dq_maps = reinterpret_cast<__half*>(ws + 3 * map_bytes);
-  float* partial = reinterpret_cast<float*>(ws + 4 * map_bytes);
-  sp.weights = p->weights;
-  sp.units = r.units(b.h, b.d);
-  sp.rows = static_cast<int>(r.rows), sp.h = b.h, sp.unit_bits = unit_bits;
-  rc = split(sp, stream);
-  if (rc != FA_OK) return rc;
-  FaBwdParams f = b;
-  f.q = sp.q_maps, f.o = sp.o_maps, f.dout = sp.do_maps, f.dq = dq_maps, f.h = 2 * b.h;
-  f.q_head_stride = f.o_head_stride = f.do_head_stride = f.dq_head_stride = b.d;
-  f.q_row_stride = f.o_row_stride = f.do_row_stride = f.dq_row_stride = static_cast<int64_t>(2) * b.h * b.d;
-  f.q_batch_stride = f.o_batch_stride = f.do_batch_stride = f.dq_batch_stride = f.q_row_stride * r.rows;
-  const size_t used = 4 * map_bytes + align256(static_cast<size_t>(b.h) * kLamChunks * 4);
-  f.workspace = ws + used, f.workspace_bytes = b.workspace_bytes - used;
-  rc = fa_bwd(&f, stream);
-  if (rc != FA_OK) return rc;
-  gather_dq_kernel<<<blocks_for(sp.units), kThreads, 0, stream>>>(dq_maps, view(b.dq, b.dq_batch_stride, b.dq_row_stride, b.dq_head_stride),
-                                                                  sp.units, sp.rows, b.h, unit_bits);
-  FA_CHECK_CUDA(cudaGetLastError());
-  const LamParams lp{sp.o2, sp.dout, partial, p->dlam, r.batches * r.rows, sp.rows, b.h, unit_bits, p->weights.is_half,
-                     p->weights.count == 1, b.cu_seqlens_q, b.b};
-  lam_partial_kernel<<<dim3(b.h, kLamChunks), kThreads, 0, stream>>>(lp);
-  FA_CHECK_CUDA(cudaGetLastError());
-  lam_sum_kernel<<<lp.one ? 1 : b.h, kThreads, 0, stream>>>(lp);
-  FA_CHECK_CUDA(cudaGetLastError());
-  return FA_OK;
 }
 
 extern "C" size_t fa_diff_kvcache_workspace_bytes(const FaDiffKvcacheParams* p) {

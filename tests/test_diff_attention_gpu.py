@@ -261,6 +261,21 @@ def test_steps_equal_the_whole_sequence():
     check(fa.flash_diff_attn_func(q, k, v, lam, causal=True)[0], want, "whole")
 
 
+def test_on_a_host_thread_of_its_own():
+    """Its first call of all is the operator's."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    gen = _gen(15)
+    q, k, v, lam = _randn(gen, 1, 140, 4, 64), _randn(gen, 1, 140, 2, 64), _randn(gen, 1, 140, 2, 64), _lam(gen, 4)
+    want = fa.flash_diff_attn_func(q, k, v, lam)
+    with ThreadPoolExecutor(1) as pool:
+        assert torch.equal(pool.submit(fa.flash_diff_attn_func, q, k, v, lam).result(), want)
+    with ThreadPoolExecutor(4) as pool:  # and several at once
+        got = list(pool.map(lambda _: fa.flash_diff_attn_func(q, k, v, lam), range(16)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
 def _training_step(gen):
     leaves = [t.requires_grad_() for t in (_randn(gen, 2, 260, 8, 64), _randn(gen, 2, 260, 2, 64), _randn(gen, 2, 260, 2, 64), _lam(gen, 8))]
     return leaves, _randn(gen, 2, 260, 8, 64)
