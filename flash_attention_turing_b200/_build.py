@@ -29,7 +29,7 @@ EXT_NAME = "_fa_b200_torch"
 EXT_PATH = PKG_DIR / f"{EXT_NAME}.so"
 
 CUDA_SOURCES = ["common.cu", "fwd_sm100.cu", "bwd_sm100.cu", "bwd_fused_sm100.cu", "kvcache_sm100.cu", "combine.cu",
-                "diff.cu", "diff_bwd_sm100.cu", "kvcache_pages.cu"]
+                "diff_bwd_sm100.cu", "kvcache_pages.cu"]
 BINDING_SOURCES = ["torch_ext.cpp", "torch_ext_pages.cpp"]
 # Ahead of the compiler's own -lstdc++, which is an archive in some installations: a second C++ runtime in the extension takes the
 # place of a part of the one torch uses, and formatting a number for an exception then crashes the process.

@@ -9,6 +9,7 @@
 // (csrc/flash_attn/src/kvcache_native.cu:676-780); rows whose every split is empty get O = 0 and
 // LSE = 0 as there (:727).
 #include "combine.h"
+#include "diff.cuh"
 
 #define FA_WAIT_INLINE
 #include "ptx.cuh"
@@ -25,15 +26,23 @@ struct CombineArgs {
   float* lse;
   int64_t rows, o_batch_stride, o_row_stride, o_head_stride;
   int num_splits, h, seqlen_q;
+  FaDiffWeights weights;  // differential
 };
 
-template <int D>
+// kDiff: rows (b, 2 * h + map, seqlen_q) of differential attention.  A block has its warps in pairs, for the two maps of a head; the
+// warp of map 2 leaves its row in shared memory, times -lam, and that of map 1 adds it and stores.
+template <int D, bool kDiff>
 __global__ void __launch_bounds__(kWarpsPerBlock * 32) combine_kernel(const __grid_constant__ CombineArgs a) {
   constexpr int kPerLane = D / 32;  // 2 or 4 consecutive columns
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5);
   grid_dependency_wait();  // the partials
-  if (row >= a.rows) return;
+  const bool beyond = row >= a.rows;
+  if (!kDiff && beyond) return;
+  if constexpr (kDiff) {  // warp 2 i + map has (batch, head, position) i of the block: row (batch, 2 * head + map, position)
+    const int64_t pair = beyond ? 0 : row >> 1;
+    row = pair / a.seqlen_q * 2 * a.seqlen_q + pair % a.seqlen_q + (row & 1) * a.seqlen_q;
+  }
 
   // log-sum-exp over splits: lanes stride over the splits, shuffles reduce
   const float* lse_row = a.lse_accum + row;
@@ -97,8 +106,27 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32) combine_kernel(const __gr
   const int q_pos = static_cast<int>(row - bh * a.seqlen_q);
   const int64_t batch = bh / a.h;
   const int head = static_cast<int>(bh - batch * a.h);
-  __half* dst = a.o + batch * a.o_batch_stride + q_pos * a.o_row_stride + head * a.o_head_stride + lane * kPerLane;
-  if constexpr (kPerLane == 4) {
+  bool stores = true;
+  if constexpr (kDiff) {
+    __shared__ float second[kWarpsPerBlock / 2][D];
+    const int warp = threadIdx.x >> 5;
+    float* mine = second[warp >> 1] + lane * kPerLane;
+    stores = (warp & 1) == 0;
+    if (!stores) {
+      const float minus = -weight_of(a.weights, head >> 1);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) mine[i] = acc[i] * minus;
+    }
+    __syncthreads();
+    if (beyond) return;
+    if (stores) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) acc[i] += mine[i];
+    }
+  }
+  __half* dst = a.o + batch * a.o_batch_stride + q_pos * a.o_row_stride + (kDiff ? head >> 1 : head) * a.o_head_stride + lane * kPerLane;
+  if (!stores) {
+  } else if constexpr (kPerLane == 4) {
     uint2 v;
     v.x = pack_half2(acc[0], acc[1]);
     v.y = pack_half2(acc[2], acc[3]);
@@ -268,14 +296,12 @@ sum_gather_kernel(const __grid_constant__ SumArgs a, __half* __restrict__ out, i
 
 }  // namespace
 
-int launch_combine(const float* o_accum, const float* lse_accum, void* o, float* lse, int64_t rows,
-                   int num_splits, int h, int seqlen_q, int d, int64_t o_batch_stride,
-                   int64_t o_row_stride, int64_t o_head_stride, cudaStream_t stream, bool overlap) {
-  if (rows == 0) return FA_OK;
-  const unsigned blocks = static_cast<unsigned>((rows + kWarpsPerBlock - 1) / kWarpsPerBlock);
-  const CombineArgs a{o_accum, lse_accum, static_cast<__half*>(o), lse, rows, o_batch_stride, o_row_stride, o_head_stride,
-                      num_splits, h, seqlen_q};
-  const auto kernel = d == 128 ? combine_kernel<128> : combine_kernel<64>;
+namespace {
+template <bool kDiff>
+int launch(const CombineArgs& a, int d, bool overlap, cudaStream_t stream) {
+  if (a.rows == 0) return FA_OK;
+  const unsigned blocks = static_cast<unsigned>((a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock);
+  const auto kernel = d == 128 ? combine_kernel<128, kDiff> : combine_kernel<64, kDiff>;
   if (overlap) {
     FA_CHECK_CUDA(launch_overlapped(kernel, dim3(blocks), kWarpsPerBlock * 32, 0, stream, a));
     return FA_OK;
@@ -283,6 +309,23 @@ int launch_combine(const float* o_accum, const float* lse_accum, void* o, float*
   kernel<<<blocks, kWarpsPerBlock * 32, 0, stream>>>(a);
   FA_CHECK_CUDA(cudaGetLastError());
   return FA_OK;
+}
+}  // namespace
+
+int launch_combine(const float* o_accum, const float* lse_accum, void* o, float* lse, int64_t rows,
+                   int num_splits, int h, int seqlen_q, int d, int64_t o_batch_stride,
+                   int64_t o_row_stride, int64_t o_head_stride, cudaStream_t stream, bool overlap) {
+  return launch<false>(CombineArgs{o_accum, lse_accum, static_cast<__half*>(o), lse, rows, o_batch_stride, o_row_stride, o_head_stride,
+                                   num_splits, h, seqlen_q, {}},
+                       d, overlap, stream);
+}
+
+int launch_diff_combine(const float* o_accum, const float* lse_accum, void* o, float* lse, int64_t rows,
+                        int num_splits, int h, int seqlen_q, int d, int64_t o_batch_stride, int64_t o_row_stride, int64_t o_head_stride,
+                        const FaDiffWeights& weights, cudaStream_t stream) {
+  return launch<true>(CombineArgs{o_accum, lse_accum, static_cast<__half*>(o), lse, rows, o_batch_stride, o_row_stride, o_head_stride,
+                                  num_splits, h, seqlen_q, weights},
+                      d, true, stream);
 }
 
 }  // namespace fa

@@ -1022,3 +1022,17 @@ int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool o
 extern "C" int fa_fwd(const FaFwdParams* p, fa_stream_t stream) {
   return fa::run_fwd(p, 0, static_cast<cudaStream_t>(stream));
 }
+
+extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream) {
+  using namespace fa;
+  FA_CHECK_ARG(p != nullptr, "fa_diff_fwd: params is NULL");
+  const FaFwdParams& b = p->base;
+  FA_CHECK_ARG(b.q && b.k && b.v && b.o && b.lse, "fa_diff_fwd: q, k, v, o, lse must be non-NULL");
+  if (b.d != 64 && b.d != 128) return set_error(FA_ERR_UNSUPPORTED, "fa_diff_fwd: head_dim must be 64 or 128");
+  FA_CHECK_ARG(b.b >= 1 && b.h >= 1 && b.h_k >= 1 && b.h % b.h_k == 0, "fa_diff_fwd: bad b / h / h_k");
+  const int rc = check_weights(p->weights, b.h, "fa_diff_fwd");
+  if (rc != FA_OK) return rc;
+  FA_CHECK_ARG(aligned16(p->o2) && p->o2_batch_stride % 8 == 0 && p->o2_row_stride % 8 == 0 && p->o2_head_stride % 8 == 0,
+               "fa_diff_fwd: o2 must be 16-byte aligned with strides that are multiples of 8 elements");
+  return run_fwd(&b, 0, static_cast<cudaStream_t>(stream), false, false, p);
+}

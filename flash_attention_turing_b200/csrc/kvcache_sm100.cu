@@ -21,10 +21,15 @@
 // split heuristic choose_num_splits (kvcache_native.cu:913-952).  Query blocks with more than 16
 // (position, head) rows per KV head go to the tiled tcgen05 forward kernel instead (the reference
 // routes them to its tiled kernel too, flash_api.cpp:668-714).
+//
+// Differential attention (kDiff): a query head is two rows of the M dimension, 2 * head + map, whose other half of d is zero, so
+// that K and V are read once for both maps and everything up to the normalised rows is as for two heads (`h` and `group` count
+// rows, and so do the partials and the LSE).  Where a row is stored, its pair is: the warp that has both subtracts them in 32 bits.
 #include <algorithm>
 #include <mutex>
 
 #include "combine.h"
+#include "diff.cuh"
 #include "fwd.h"
 #define FA_WAIT_INLINE  // two roles with a few waits each: code size is no concern here
 #include "ptx.cuh"
@@ -64,7 +69,14 @@ struct DecodeParams {
   int b;             // sequences
   int* arrivals;     // balanced kernel: a counter per CTA in scratch memory, zeroed by the kernel before
   int* status;
+  FaDiffWeights weights;  // differential
 };
+
+// Where row `head` (differential: 2 * head + map) of the output is
+template <bool kDiff>
+__device__ __forceinline__ __half* out_row(const DecodeParams& p, int batch, int q_pos, int head) {
+  return p.o + batch * p.o_batch_stride + q_pos * p.o_row_stride + (kDiff ? head >> 1 : head) * p.o_head_stride;
+}
 
 template <int D>
 struct DCfg {
@@ -120,7 +132,7 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c8) {
 }
 
 // What a consumer warp holds of its (up to 16) query rows: the Q fragments and the running (maximum, sum, O) over its tokens.
-template <int D>
+template <int D, bool kDiff>
 struct WarpRows {
   uint32_t qa[D / 16][4];
   int lim0, lim1;         // last visible key of fragment rows g and g + 8
@@ -128,21 +140,29 @@ struct WarpRows {
   float m0, m1;           // reference maxima (raw score units)
   float l0, l1;           // per-thread partial row sums
 
-  __device__ __forceinline__ void begin(const DecodeParams& p, int batch, int head_k, int len, int rows, int lane) {
+  // first: the row of the KV head that is row 0 here
+  __device__ __forceinline__ void begin(const DecodeParams& p, int batch, int head_k, int len, int first, int rows, int lane) {
     const int g = lane >> 2;   // fragment row (and row + 8)
     const int t4 = lane & 3;   // fragment column pair
     // Q fragments (A operand, 16 x D), straight from global memory; rows >= `rows` are zero.
     {
       auto q_ptr = [&](int r) -> const __half* {
+        r += first;
         const int q_pos = r / p.group;
         const int head = head_k * p.group + (r - q_pos * p.group);
-        return p.q + batch * p.q_batch_stride + q_pos * p.q_row_stride + head * p.q_head_stride;
+        return p.q + batch * p.q_batch_stride + q_pos * p.q_row_stride + (kDiff ? head >> 1 : head) * p.q_head_stride;
       };
+      // differential: the half of d that a row has (groups are even, so rows g and g + 8 have the same)
+      const int map = (first + g) & 1;
       const __half* r0p = g < rows ? q_ptr(g) : nullptr;
       const __half* r1p = (g + 8) < rows ? q_ptr(g + 8) : nullptr;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const int c = k * 16 + t4 * 2;
+        if (kDiff && k / (D / 32) != map) {
+          qa[k][0] = qa[k][1] = qa[k][2] = qa[k][3] = 0u;
+          continue;
+        }
         qa[k][0] = r0p ? *reinterpret_cast<const uint32_t*>(r0p + c) : 0u;
         qa[k][1] = r1p ? *reinterpret_cast<const uint32_t*>(r1p + c) : 0u;
         qa[k][2] = r0p ? *reinterpret_cast<const uint32_t*>(r0p + c + 8) : 0u;
@@ -152,8 +172,8 @@ struct WarpRows {
     // causal limit per fragment row: key j visible iff j <= q_pos + len - seqlen_q
     lim0 = lim1 = len - 1;
     if (p.is_causal) {
-      lim0 = min(lim0, g / p.group + len - p.seqlen_q);
-      lim1 = min(lim1, (g + 8) / p.group + len - p.seqlen_q);
+      lim0 = min(lim0, (first + g) / p.group + len - p.seqlen_q);
+      lim1 = min(lim1, (first + g + 8) / p.group + len - p.seqlen_q);
     }
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
@@ -254,17 +274,19 @@ struct WarpRows {
   }
 };
 
-template <int D>
+template <int D, bool kDiff>
 __global__ void __launch_bounds__(kDecodeThreads, (D == 128) ? 2 : 2)
 decode_split_kernel(const __grid_constant__ DecodeParams p) {
   using C = DCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   const int split = blockIdx.x;
-  const int head_k = blockIdx.y;
+  // differential: more than 16 rows are several M tiles, each with CTAs of its own
+  const int first_row = kDiff ? static_cast<int>(blockIdx.y) / p.h_k * kMaxRows : 0;
+  const int head_k = kDiff ? static_cast<int>(blockIdx.y) % p.h_k : blockIdx.y;
   const int batch = blockIdx.z;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rows = p.seqlen_q * p.group;  // valid rows of the 16-row M tile
+  const int rows = kDiff ? min(p.seqlen_q * p.group - first_row, kMaxRows) : p.seqlen_q * p.group;  // valid rows of the 16-row M tile
   grid_launch_dependents();  // the merge waits for this grid by itself
 
   // ---- this CTA's token range ----
@@ -286,6 +308,7 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
 
   // row r of the M tile -> (query position, head); output row index in (b, h, seqlen_q) order
   auto out_row_index = [&](int r) -> int64_t {
+    r += first_row;
     const int q_pos = r / p.group;
     const int head = head_k * p.group + (r - q_pos * p.group);
     return (static_cast<int64_t>(batch) * p.h + head) * p.seqlen_q + q_pos;
@@ -303,11 +326,10 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
         float2* dst = reinterpret_cast<float2*>(p.o_accum + (split * p.rows_total + orow) * D + c);
         *dst = make_float2(0.f, 0.f);
       } else {
-        const int q_pos = r / p.group;
-        const int head = head_k * p.group + (r - q_pos * p.group);
-        __half2* dst = reinterpret_cast<__half2*>(p.o + batch * p.o_batch_stride + q_pos * p.o_row_stride +
-                                                  head * p.o_head_stride + c);
-        *dst = __floats2half2_rn(0.f, 0.f);
+        const int q_pos = (first_row + r) / p.group;
+        const int head = head_k * p.group + (first_row + r - q_pos * p.group);
+        __half2* dst = reinterpret_cast<__half2*>(out_row<kDiff>(p, batch, q_pos, head) + c);
+        *dst = __floats2half2_rn(0.f, 0.f);  // differential: twice the same zero
       }
     }
     for (int r = threadIdx.x; r < rows; r += blockDim.x) {
@@ -364,8 +386,8 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
     // =========================== consumers ===========================
     const int g = lane >> 2;   // fragment row (and row + 8)
     const int t4 = lane & 3;   // fragment column pair
-    WarpRows<D> w;
-    w.begin(p, batch, head_k, len, rows, lane);
+    WarpRows<D, kDiff> w;
+    w.begin(p, batch, head_k, len, first_row, rows, lane);
     const float c = p.scale_log2;
     const int tok_in_tile = warp * 16;     // this warp's 16 tokens of every tile
     bool ok = true;
@@ -415,7 +437,8 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
       const int tid = threadIdx.x;
       const int r = tid / kThreadsPerRow;
       const int c0 = (tid - r * kThreadsPerRow) * kColsPerThread;
-      if (r < rows) {
+      // differential: a row's pair is in the lanes eight further on; all rows go through, those behind the last one are not stored
+      if (kDiff || r < rows) {
         float mw[kConsumerWarps], lw[kConsumerWarps];
         float mt = -INFINITY;
 #pragma unroll
@@ -443,7 +466,31 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
         }
         const float lse_val = dead ? -INFINITY : (mt * c + __log2f(lt)) * kLn2;
         const int64_t orow = out_row_index(r);
-        if (p.num_splits > 1) {
+        if constexpr (kDiff) {
+          if (p.num_splits == 1) {
+            const int q_pos = (first_row + r) / p.group;
+            const int head = head_k * p.group + (first_row + r - q_pos * p.group);
+            const float minus = r < rows ? -weight_of(p.weights, head >> 1) : 0.f;
+            float v[kColsPerThread];
+#pragma unroll
+            for (int j = 0; j < kColsPerThread; ++j) {
+              const float x = dead ? 0.f : acc[j] * inv;  // no visible key: 0 times a value that is hidden may be NaN
+              v[j] = fmaf(minus, __shfl_down_sync(0xffffffffu, x, kThreadsPerRow), x);
+            }
+            if (r < rows) {
+              if ((r & 1) == 0) {
+                __half* dst = out_row<true>(p, batch, q_pos, head) + c0;
+#pragma unroll
+                for (int j = 0; j < kColsPerThread; j += 8)
+                  *reinterpret_cast<uint4*>(dst + j) = make_uint4(pack_half2(v[j], v[j + 1]), pack_half2(v[j + 2], v[j + 3]),
+                                                                  pack_half2(v[j + 4], v[j + 5]), pack_half2(v[j + 6], v[j + 7]));
+              }
+              if (c0 == 0) p.lse[orow] = dead ? 0.f : lse_val;
+            }
+          }
+        }
+        if (kDiff && (r >= rows || p.num_splits == 1)) {
+        } else if (p.num_splits > 1) {
           float* dst = p.o_accum + (split * p.rows_total + orow) * D + c0;
 #pragma unroll
           for (int j = 0; j < kColsPerThread; j += 4)
@@ -653,7 +700,7 @@ __device__ __forceinline__ float merge_row(const float* o_accum, const float* ls
   return dead ? 0.f : mx + __logf(sum);
 }
 
-template <int D>
+template <int D, bool kDiff>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
   using C = DCfg<D>;
@@ -703,8 +750,7 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
       for (int idx = threadIdx.x; idx < rows * (D / 8); idx += blockDim.x) {
         int q_pos;
         const int head = row_head(idx / (D / 8), q_pos);
-        *reinterpret_cast<uint4*>(p.o + w.batch * p.o_batch_stride + q_pos * p.o_row_stride + head * p.o_head_stride +
-                                  idx % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(out_row<kDiff>(p, w.batch, q_pos, head) + idx % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
         if (idx % (D / 8) == 0) p.lse[(static_cast<int64_t>(w.batch) * p.h + head) * p.seqlen_q + q_pos] = 0.f;
       }
     }
@@ -771,8 +817,8 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
       if (w.tile == 0 && head_k == 0 && threadIdx.x == 0 && p.status &&
           cache_length(p.cache_seqlens[w.batch], p.seqlen_new, p.capacity, p.checked).report)
         atomicOr(p.status, kStatusCapacityClamped);
-      WarpRows<D> mine;
-      mine.begin(p, w.batch, head_k, w.len, rows, lane);
+      WarpRows<D, kDiff> mine;
+      mine.begin(p, w.batch, head_k, w.len, 0, rows, lane);
       for (int t = 0; t < n; ++t, ++i) {
         if (!(ok = wait_full(i))) break;
         uint8_t* stage = smem + (i % C::kStages) * C::kStageBytes;
@@ -802,54 +848,72 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
       // would be at the end of the kernel while the others wait for it at this barrier, without a limit).
       if (!(ok = named_barrier_and(1, kConsumerWarps * 32, ok))) break;
 
-      // a warp per row, a lane per kPerLane columns
+      // a warp per row (differential: per pair of rows), a lane per kPerLane columns
+      constexpr int kRowsAtOnce = kDiff ? 2 : 1;
       auto store = [&](int r, const float (&acc)[kPerLane], float mul, float lse) {
         int q_pos;
         const int head = row_head(r, q_pos);
-        __half* out = p.o + w.batch * p.o_batch_stride + q_pos * p.o_row_stride + head * p.o_head_stride + lane * kPerLane;
-        if constexpr (kPerLane == 4) {
+        __half* out = out_row<kDiff>(p, w.batch, q_pos, head) + lane * kPerLane;
+        if (kDiff && (r & 1) != 0) {  // stored with its pair
+        } else if constexpr (kPerLane == 4) {
           *reinterpret_cast<uint2*>(out) = make_uint2(pack_half2(acc[0] * mul, acc[1] * mul), pack_half2(acc[2] * mul, acc[3] * mul));
         } else {
           *reinterpret_cast<uint32_t*>(out) = pack_half2(acc[0] * mul, acc[1] * mul);
         }
         if (lane == 0) p.lse[(static_cast<int64_t>(w.batch) * p.h + head) * p.seqlen_q + q_pos] = lse;
       };
+      // differential: the row of map 2 times -lam, to be added to that of map 1
+      auto minus = [&](int r) {
+        int q_pos;
+        return -weight_of(p.weights, row_head(r, q_pos) >> 1);
+      };
       // part of a sequence in scratch memory: slot 1 of the CTA where the sequence begins, slot 0 of the others
       auto part = [&](int owner, bool begins) { return 2 * (owner * static_cast<int>(gridDim.x) + head_k) + (begins ? 1 : 0); };
-      for (int r = warp; r < rows; r += kConsumerWarps) {
-        float2 of[kConsumerWarps];
-        float mt = -INFINITY;
+      for (int r0 = warp * kRowsAtOnce; r0 < rows; r0 += kConsumerWarps * kRowsAtOnce) {
+        float other[kPerLane];  // differential: the row of map 2, which is merged first
+#pragma unroll 1
+        for (int r = r0 + kRowsAtOnce - 1; r >= r0; --r) {
+          float2 of[kConsumerWarps];
+          float mt = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kConsumerWarps; ++u) {
-          of[u] = ml[u * kBalancedRows + r];
-          mt = fmaxf(mt, of[u].x);
-        }
-        float lt = 0.f, acc[kPerLane];
-#pragma unroll
-        for (int e = 0; e < kPerLane; ++e) acc[e] = 0.f;
-        const int col = (lane * kPerLane) ^ ((r & 7) * 8);
-#pragma unroll
-        for (int u = 0; u < kConsumerWarps; ++u) {
-          const float scale = of[u].x == -INFINITY ? 0.f : ex2f((of[u].x - mt) * c);
-          lt += of[u].y * scale;
-          float x[kPerLane];
-          load_floats(mbuf + (u * kBalancedRows + r) * D + col, x);
-#pragma unroll
-          for (int e = 0; e < kPerLane; ++e) acc[e] = fmaf(x[e], scale, acc[e]);
-        }
-        const bool dead = mt == -INFINITY || lt == 0.f;
-        if (dead) {  // no visible key: 0 times a value that is hidden may be NaN
+          for (int u = 0; u < kConsumerWarps; ++u) {
+            of[u] = ml[u * kBalancedRows + r];
+            mt = fmaxf(mt, of[u].x);
+          }
+          float lt = 0.f, acc[kPerLane];
 #pragma unroll
           for (int e = 0; e < kPerLane; ++e) acc[e] = 0.f;
-        }
-        const float inv = dead ? 0.f : 1.f / lt;
-        const float lse = dead ? -INFINITY : (mt * c + __log2f(lt)) * kLn2;
-        if (whole) {
-          store(r, acc, inv, dead ? 0.f : lse);
-        } else {
-          const int slot = part(cta, w.tile == 0);
-          store_floats(p.o_accum + (static_cast<int64_t>(slot) * kBalancedRows + r) * D + lane * kPerLane, acc, inv);
-          if (lane == 0) p.lse_accum[slot * kBalancedRows + r] = lse;
+          const int col = (lane * kPerLane) ^ ((r & 7) * 8);
+#pragma unroll
+          for (int u = 0; u < kConsumerWarps; ++u) {
+            const float scale = of[u].x == -INFINITY ? 0.f : ex2f((of[u].x - mt) * c);
+            lt += of[u].y * scale;
+            float x[kPerLane];
+            load_floats(mbuf + (u * kBalancedRows + r) * D + col, x);
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) acc[e] = fmaf(x[e], scale, acc[e]);
+          }
+          const bool dead = mt == -INFINITY || lt == 0.f;
+          if (dead) {  // no visible key: 0 times a value that is hidden may be NaN
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) acc[e] = 0.f;
+          }
+          const float inv = dead ? 0.f : 1.f / lt;
+          const float lse = dead ? -INFINITY : (mt * c + __log2f(lt)) * kLn2;
+          if (!whole) {
+            const int slot = part(cta, w.tile == 0);
+            store_floats(p.o_accum + (static_cast<int64_t>(slot) * kBalancedRows + r) * D + lane * kPerLane, acc, inv);
+            if (lane == 0) p.lse_accum[slot * kBalancedRows + r] = lse;
+          } else if constexpr (kDiff) {
+            const float f = r == r0 ? inv : inv * minus(r);
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) acc[e] = r == r0 ? fmaf(acc[e], f, other[e]) : acc[e] * f;
+#pragma unroll
+            for (int e = 0; e < kPerLane; ++e) other[e] = acc[e];
+            store(r, acc, 1.f, dead ? 0.f : lse);
+          } else {
+            store(r, acc, inv, dead ? 0.f : lse);
+          }
         }
       }
       if (!whole) {
@@ -863,10 +927,21 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
         }
         named_barrier_sync(1, kConsumerWarps * 32);
         if (bars->last) {
-          for (int r = warp; r < rows; r += kConsumerWarps) {
-            float acc[kPerLane];
-            const float lse = merge_row<D>(p.o_accum, p.lse_accum, part(c0, true), gridDim.x, parts, r, mbuf + warp * kPartsAtOnce * D, lane, acc);
-            store(r, acc, 1.f, lse);
+          for (int r0 = warp * kRowsAtOnce; r0 < rows; r0 += kConsumerWarps * kRowsAtOnce) {
+            float other[kPerLane];
+#pragma unroll 1
+            for (int r = r0 + kRowsAtOnce - 1; r >= r0; --r) {
+              float acc[kPerLane];
+              const float lse = merge_row<D>(p.o_accum, p.lse_accum, part(c0, true), gridDim.x, parts, r, mbuf + warp * kPartsAtOnce * D, lane, acc);
+              if constexpr (kDiff) {
+                const float f = r == r0 ? 1.f : minus(r);
+#pragma unroll
+                for (int e = 0; e < kPerLane; ++e) acc[e] = r == r0 ? acc[e] + other[e] : acc[e] * f;
+#pragma unroll
+                for (int e = 0; e < kPerLane; ++e) other[e] = acc[e];
+              }
+              store(r, acc, 1.f, lse);
+            }
           }
         }
       }
@@ -990,9 +1065,13 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   }
 }
 
-bool uses_decode_kernel(const FaKvcacheParams* p) {
-  return static_cast<int64_t>(p->seqlen_q) * (p->h / p->h_k) <= kMaxRows;
+// Differential calls (p->h counts two rows per head then) of up to kMaxDiffRows rows go to the split kernel, whose M tiles read the
+// keys from L2 after the first: the tiled kernel has a CTA per head and no split.
+constexpr int kMaxDiffRows = 64;
+bool uses_decode_kernel(const FaKvcacheParams* p, bool diff) {
+  return static_cast<int64_t>(p->seqlen_q) * (p->h / p->h_k) <= (diff ? kMaxDiffRows : kMaxRows);
 }
+int row_tiles(const FaKvcacheParams* p) { return (p->seqlen_q * (p->h / p->h_k) + kMaxRows - 1) / kMaxRows; }
 
 int capacity_tokens(const FaKvcacheParams* p) {
   return p->block_table ? p->max_blocks_per_seq * p->seqlen_cache : p->seqlen_cache;
@@ -1080,9 +1159,9 @@ struct Plan {
   size_t lse = 0;         // scratch memory: offset of the LSE of the parts behind the parts, and the size
   size_t bytes = 0;
 };
-Plan plan_call(const FaKvcacheParams* p) {
+Plan plan_call(const FaKvcacheParams* p, bool diff = false) {
   Plan plan;
-  if (!uses_decode_kernel(p)) return plan;
+  if (!uses_decode_kernel(p, diff)) return plan;
   if (p->num_splits > 0) {
     plan.splits = std::min(p->num_splits, 256);
   } else {
@@ -1159,8 +1238,10 @@ extern "C" size_t fa_kvcache_workspace_bytes(const FaKvcacheParams* p) {
 
 namespace fa {
 namespace {
-// verdict: see fa_kvcache_checked(); NULL: lengths are clamped to the capacity
-int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t stream) {
+// verdict: see fa_kvcache_checked(); NULL: lengths are clamped to the capacity.  weights: differential attention, and p->h counts two
+// rows per query head; else NULL.
+int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* verdict, int token, cudaStream_t stream) {
+  const bool diff = weights != nullptr;
   int rc = validate(p, "fa_kvcache");
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(p->q && p->k_cache && p->v_cache && p->o && p->lse && p->cache_seqlens,
@@ -1174,7 +1255,7 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
   rc = check_device_sm100();
   if (rc != FA_OK) return rc;
 
-  Plan plan = plan_call(p);
+  Plan plan = plan_call(p, diff);
   uint8_t* scratch = nullptr;
   if (plan.bytes > 0) {
     const bool enough = p->workspace != nullptr && p->workspace_bytes >= plan.bytes;
@@ -1233,9 +1314,10 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
   }
 
   // ---- 2. attend ----
-  if (!uses_decode_kernel(p)) {
+  if (!uses_decode_kernel(p, diff)) {
     // many query rows per KV head: tiled tcgen05 forward over the cache
-    FaFwdParams f = {};
+    FaDiffFwdParams tiled = {};
+    FaFwdParams& f = tiled.base;
     f.q = p->q; f.k = p->k_cache; f.v = p->v_cache; f.o = p->o; f.lse = p->lse;
     f.q_batch_stride = p->q_batch_stride; f.q_row_stride = p->q_row_stride; f.q_head_stride = p->q_head_stride;
     f.k_batch_stride = p->kc_batch_stride; f.k_row_stride = p->kc_row_stride; f.k_head_stride = p->kc_head_stride;
@@ -1243,7 +1325,7 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
     f.o_batch_stride = p->o_batch_stride; f.o_row_stride = p->o_row_stride; f.o_head_stride = p->o_head_stride;
     f.lse_row_stride = p->seqlen_q;
     f.b = p->b; f.seqlen_q = p->seqlen_q; f.seqlen_k = p->seqlen_cache;
-    f.h = p->h; f.h_k = p->h_k; f.d = p->d;
+    f.h = diff ? p->h / 2 : p->h; f.h_k = p->h_k; f.d = p->d;
     f.k_batch = p->cache_batch;
     f.softmax_scale = p->softmax_scale; f.is_causal = p->is_causal;
     f.seqused_k = p->cache_seqlens;
@@ -1252,7 +1334,8 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
     f.block_table_batch_stride = p->block_table_batch_stride;
     f.page_size = p->block_table ? p->seqlen_cache : 0;
     f.block_table_cols = p->block_table ? p->max_blocks_per_seq : 0;
-    return run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr);
+    if (diff) tiled.weights = *weights;
+    return run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr, diff ? &tiled : nullptr);
   }
 
   const int64_t rows_total = static_cast<int64_t>(p->b) * p->h * p->seqlen_q;
@@ -1289,18 +1372,30 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
   dp.arrivals = arrivals;
   dp.checked = verdict != nullptr;
   dp.status = device_status_ptr();
+  dp.weights = diff ? *weights : FaDiffWeights{};
   if (plan.balanced) {
     const dim3 grid(p->h_k, balanced_shares(p));
     const bool overlap = appends || num_arrivals > 0;
-    return p->d == 128 ? launch_decode<128, decode_balanced_kernel<128>>(dp, grid, overlap, stream)
-                       : launch_decode<64, decode_balanced_kernel<64>>(dp, grid, overlap, stream);
+    if (diff)
+      return p->d == 128 ? launch_decode<128, decode_balanced_kernel<128, true>>(dp, grid, overlap, stream)
+                         : launch_decode<64, decode_balanced_kernel<64, true>>(dp, grid, overlap, stream);
+    return p->d == 128 ? launch_decode<128, decode_balanced_kernel<128, false>>(dp, grid, overlap, stream)
+                       : launch_decode<64, decode_balanced_kernel<64, false>>(dp, grid, overlap, stream);
   }
-  const dim3 grid(plan.splits, p->h_k, p->b);
-  rc = p->d == 128 ? launch_decode<128, decode_split_kernel<128>>(dp, grid, appends, stream)
-                   : launch_decode<64, decode_split_kernel<64>>(dp, grid, appends, stream);
+  const dim3 grid(plan.splits, diff ? p->h_k * row_tiles(p) : p->h_k, p->b);
+  if (diff) {
+    rc = p->d == 128 ? launch_decode<128, decode_split_kernel<128, true>>(dp, grid, appends, stream)
+                     : launch_decode<64, decode_split_kernel<64, true>>(dp, grid, appends, stream);
+  } else {
+    rc = p->d == 128 ? launch_decode<128, decode_split_kernel<128, false>>(dp, grid, appends, stream)
+                     : launch_decode<64, decode_split_kernel<64, false>>(dp, grid, appends, stream);
+  }
   if (rc != FA_OK) return rc;
 
   // ---- 3. merge ----
+  if (plan.splits > 1 && diff)
+    return launch_diff_combine(dp.o_accum, dp.lse_accum, p->o, p->lse, rows_total, plan.splits, p->h, p->seqlen_q, p->d,
+                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, stream);
   if (plan.splits > 1)
     return launch_combine(dp.o_accum, dp.lse_accum, p->o, p->lse, rows_total, plan.splits, p->h, p->seqlen_q, p->d,
                           p->o_batch_stride, p->o_row_stride, p->o_head_stride, stream, true);
@@ -1310,13 +1405,35 @@ int run_kvcache(const FaKvcacheParams* p, int* verdict, int token, cudaStream_t 
 }  // namespace fa
 
 extern "C" int fa_kvcache(const FaKvcacheParams* p, fa_stream_t stream) {
-  return fa::run_kvcache(p, nullptr, 0, static_cast<cudaStream_t>(stream));
+  return fa::run_kvcache(p, nullptr, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fa_kvcache_checked(const FaKvcacheParams* p, int32_t* verdict, int32_t token, fa_stream_t stream) {
   using namespace fa;
   FA_CHECK_ARG(verdict != nullptr && token >= 0 && token < (1 << 30), "fa_kvcache_checked: verdict is NULL or token out of range");
-  return run_kvcache(p, verdict, token, static_cast<cudaStream_t>(stream));
+  return run_kvcache(p, nullptr, verdict, token, static_cast<cudaStream_t>(stream));
+}
+
+// The calls of differential attention, with h doubled for the kernels (see run_kvcache)
+extern "C" size_t fa_diff_kvcache_workspace_bytes(const FaDiffKvcacheParams* p) {
+  using namespace fa;
+  if (p == nullptr || p->base.h < 1 || p->base.h >= (1 << 30) || validate(&p->base, "fa_diff_kvcache_workspace_bytes") != FA_OK) return 0;
+  FaKvcacheParams rows = p->base;
+  rows.h *= 2;
+  return plan_call(&rows, true).bytes;
+}
+
+extern "C" int fa_diff_kvcache(const FaDiffKvcacheParams* p, int32_t* verdict, int32_t token, fa_stream_t stream) {
+  using namespace fa;
+  FA_CHECK_ARG(p != nullptr, "fa_diff_kvcache: params is NULL");
+  int rc = validate(&p->base, "fa_diff_kvcache");
+  if (rc == FA_OK) rc = check_weights(p->weights, p->base.h, "fa_diff_kvcache");
+  if (rc != FA_OK) return rc;
+  FA_CHECK_ARG(p->base.h < (1 << 30), "fa_diff_kvcache: too many heads");
+  FA_CHECK_ARG(verdict == nullptr || (token >= 0 && token < (1 << 30)), "fa_diff_kvcache: token out of range");
+  FaKvcacheParams rows = p->base;
+  rows.h *= 2;
+  return run_kvcache(&rows, &p->weights, verdict, token, static_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------------------------------------

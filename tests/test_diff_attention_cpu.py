@@ -57,6 +57,8 @@ def test_c_entry_points_check_their_arguments():
     assert lib.fa_diff_kvcache(None, None, 0, None) == -1
     assert lib.fa_diff_fwd(ctypes.byref(f), None) == -1 and b"non-NULL" in lib.fa_last_error()
     assert lib.fa_diff_bwd(ctypes.byref(b), None) == -1
+    assert lib.fa_diff_kvcache(ctypes.byref(k), None, 0, None) == -2  # d, as fa_kvcache()
+    k.base.d = 64
     assert lib.fa_diff_kvcache(ctypes.byref(k), None, 0, None) == -1
     at = 1 << 20  # an address that is never read: the call ends before
     f.base.q = f.base.k = f.base.v = f.base.o = f.base.lse = at

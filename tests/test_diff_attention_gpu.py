@@ -193,6 +193,12 @@ CACHE = [  # b, new, q rows, lengths, h, hk, d, page (0: contiguous), num_splits
     (2, 3, 3, [40, 4000], 8, 8, 128, 512, 1),
     (3, 130, 130, [1, 300, 77], 4, 2, 64, 256, 0),  # a chunk of a prompt
     (2, 257, 257, [0, 511], 8, 2, 128, 256, 0),
+    (2, 3, 3, [1500, 20], 16, 4, 128, 256, 0),    # 24 rows per KV head: two M tiles
+    (1, 7, 7, [3001], 8, 2, 64, 0, 0),            # 56 rows, the last tile half full
+    (3, 5, 5, [0, 130, 2], 6, 1, 128, 0, 4),      # 60 rows, groups of three
+    (2, 8, 8, [700, 1], 8, 2, 64, 256, 1),        # 64 rows, one split
+    (2, 9, 9, [700, 1], 8, 2, 64, 256, 0),        # 72 rows: the tiled kernel
+    (1, 4, 4, [50000], 2, 1, 128, 0, 0),          # a long cache, shared out over many CTAs
     (64, 1, 1, list(range(5, 645, 10)), 4, 2, 64, 256, 0),
     (40, 1, 1, list(range(100, 4100, 100)), 8, 4, 128, 256, 0),
 ]
