@@ -7,9 +7,17 @@ namespace fa {
 
 // Same as fa_fwd(); seqused_k_add is added to every seqused_k[b] on the device.  overlap: the previous kernel of the stream
 // lets this one start early (launch_overlapped).  checked: the host refuses lengths beyond the capacity; they are neither read nor
-// reported.  diff: differential attention, with p = &diff->base.
+// reported.  diff: differential attention, with p = &diff->base.  parts: with diff, and queries that are not packed; O and the LSE are
+// then not written.
+struct DiffSplits {
+  int splits = 1;
+  int chunk = 1 << 24;         // 128-key blocks of a part
+  int64_t rows = 0;            // b * 2 h * seqlen_q
+  float* o_accum = nullptr;    // (splits, rows, d), normalised
+  float* lse_accum = nullptr;  // (splits, rows), -inf: nothing there
+};
 int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap = false, bool checked = false,
-            const FaDiffFwdParams* diff = nullptr);
+            const FaDiffFwdParams* diff = nullptr, const DiffSplits* parts = nullptr);
 
 #ifdef __CUDACC__
 // What a sequence of a cache holds, limited to what it can hold; in 64 bits, a length may be any int32.  Beyond the capacity:

@@ -96,6 +96,7 @@ struct FwdKernelParams {
   FaDiffWeights weights;
   __half* o2;         // A_2 V, or null
   int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
+  DiffSplits parts;   // splits > 1: the keys of a row tile are several items, which leave partial rows
 };
 
 template <int D>
@@ -122,7 +123,7 @@ struct __align__(16) Work {
   int k_off, bq, bk, nkb;
   int fix_v_tail;
   float lam;  // differential: the weight of the head
-  int pad[2];
+  int j0, split;  // differential: the item's first key block, and its place among those of the rows
 };
 
 struct Barriers {
@@ -154,7 +155,7 @@ static_assert(sizeof(Barriers) <= 1024, "barrier block");
 static_assert((kNumThreads / 32 + 3) / 4 * 32 * 168 <= 16384, "register file of one SM sub-partition");
 
 template <int D, int kItemRows, bool kDiff>
-__device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, int head, int mpair, Work& w) {
+__device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, int head, int mpair, int split, Work& w) {
   w.mpair = mpair;
   w.batch = batch;
   w.head = head;
@@ -186,6 +187,10 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
       n = x <= 0 ? 0 : min(w.nkb, (x + kBlockN - 1) / kBlockN);
     }
     if (r0 >= w.sq) n = 0;
+    if constexpr (kDiff) {
+      w.split = split, w.j0 = split * p.parts.chunk;
+      n = max(0, min(n - w.j0, p.parts.chunk));
+    }
     w.nb[t] = n;
   }
   w.nb_max = max(w.nb[0], w.nb[1]);
@@ -194,7 +199,8 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
   // masked, but P = 0 times a NaN/Inf bit pattern in V would still poison O, so those V rows are zeroed
   // in shared memory before the last PV MMA.  (Dense tensors: TMA fills out-of-range rows with zeros.)
   if constexpr (kDiff) w.lam = weight_of(p.weights, head);
-  w.fix_v_tail = (p.seqused_k != nullptr || varlen_k) && (w.sk % kBlockN) != 0 && w.nb_max == w.nkb && w.nkb > 0;
+  w.fix_v_tail = (p.seqused_k != nullptr || varlen_k) && (w.sk % kBlockN) != 0 && (kDiff ? w.nb_max > 0 && w.j0 + w.nb_max == w.nkb : w.nb_max == w.nkb) &&
+                 w.nkb > 0;
 }
 
 // kItemRows = 256: two Q tiles per item.  kItemRows = 128: one, the second tile's warps have nothing to do (dense batches, chosen
@@ -300,8 +306,12 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         Work it;
         it.mpair = -1;
         while (next < p.total_items) {
-          int batch, head, mpair;
-          if (p.cu_seqlens_q == nullptr) {
+          int batch, head, mpair, split = 0;
+          if (kDiff && p.parts.splits > 1) {  // a cache: the parts of a row tile one after the other, its longest ones first
+            const int tile = next / p.parts.splits;
+            split = next - tile * p.parts.splits;
+            batch = tile / (p.items_x * p.h), head = tile / p.items_x - batch * p.h, mpair = p.items_x - 1 - tile % p.items_x;
+          } else if (p.cu_seqlens_q == nullptr) {
             // D = 64 takes the plain order of calls without sections here.  What section_item() gives then is as good an order, but with
             // it (or with the quotient in place of p.h / p.h_k, see make_work) the softmax loop, of which nothing changes in the source, came
             // out 2-4 % slower: us, B1 S9593 H2 causal 132.2 : 126.9, B8 S1024 Hq32 Hkv2 119.1 : 116.8, B1 S8192 Hq64 Hkv8 1583 : 1540.
@@ -332,8 +342,8 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           }
           const int sq = p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q;
           if (mpair >= 0 && mpair * kItemRows < sq) {
-            make_work<D, kItemRows, kDiff>(p, batch, head, mpair, it);
-            if (p.seqused_k && p.status && head == 0 && mpair == 0 &&
+            make_work<D, kItemRows, kDiff>(p, batch, head, mpair, split, it);
+            if (p.seqused_k && p.status && head == 0 && mpair == 0 && split == 0 &&
                 cache_length(p.seqused_k[batch], p.seqused_k_add, p.k_capacity, p.checked).report)
               atomicOr(p.status, kStatusCapacityClamped);
             break;
@@ -391,10 +401,11 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           const int gj = g + j;
           const int s = gj % C::kStages;
           const uint32_t ph = (gj / C::kStages) & 1;
-          int krow = w.k_off + j * kBlockN;
+          const int first_key = ((kDiff ? w.j0 : 0) + j) * kBlockN;
+          int krow = w.k_off + first_key;
           int kb = w.bk;
           if (p.block_table) {
-            const int tok = j * kBlockN;
+            const int tok = first_key;
             kb = p.block_table[w.batch * p.block_table_batch_stride + tok / p.page_size];
             krow = tok % p.page_size;
           }
@@ -415,7 +426,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (w.fix_v_tail) {
-        const int gj = g + w.nkb - 1;
+        const int gj = g + w.nkb - 1 - (kDiff ? w.j0 : 0);
         const int s = gj % C::kStages;
         if (!mbar_wait_warp(&bars->v_full[s], (gj / C::kStages) & 1, ctx)) break;
         // zero whole 128-byte row segments: the swizzle only permutes 16-byte units inside a row
@@ -499,7 +510,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           // V(j) and K(j+1) are not polled here: a barrier poll costs this thread 60-130 clocks in which it
           // issues nothing, so the softmax warps observe v_full / k_full while they wait for S anyway, and
           // their p_full arrival carries the observation over (mbarrier release/acquire is cumulative).
-          if (w.fix_v_tail && j == w.nkb - 1 && !(ok = mbar_wait(&bars->v_fixed[nf & 1], (nf >> 1) & 1, ctx))) break;
+          if (w.fix_v_tail && j == w.nkb - 1 - (kDiff ? w.j0 : 0) && !(ok = mbar_wait(&bars->v_fixed[nf & 1], (nf >> 1) & 1, ctx))) break;
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const int nbt = t ? nb1 : nb0;
@@ -572,6 +583,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       const volatile Work& w = bars->items[n % kSchedDepth];
       if (w.mpair < 0) break;
       const int nbt = w.nb[t], sk = w.sk, shift = w.shift, row = w.row0 + (kDiff ? 0 : t * kBlockM) + row_in_tile, nb_max = w.nb_max;
+      const int j0 = kDiff ? w.j0 : 0;
 
       float m = -INFINITY;  // lazily updated reference maximum of the row (raw score units)
       float l = 0.f;        // row sum relative to m
@@ -589,7 +601,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         tc_fence_after_sync();
 
         // masking: only blocks that touch the sequence end or the causal diagonal
-        const int col0 = j * kBlockN;
+        const int col0 = (j + j0) * kBlockN;
         int lim = sk - 1 - col0;  // last visible column index within this block
         if (p.is_causal) lim = min(lim, row + shift - col0);
         const bool masked = lim < kBlockN - 1;
@@ -710,6 +722,36 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         if (nbt > 0 && l > 0.f && m != -INFINITY) {
           inv = 1.f / l;
           lse_val = (m * c + __log2f(l)) * kLn2;
+        }
+        if (p.parts.splits > 1) {  // the map's rows over the item's keys, normalised, in 32 bits
+          const int64_t part_row = (static_cast<int64_t>(w.batch) * 2 * p.h + 2 * w.head + t) * p.seqlen_q + row +
+                                   w.split * p.parts.rows;
+          if (row_valid) p.parts.lse_accum[part_row] = inv == 0.f ? -INFINITY : lse_val;
+          if (nbt > 0) {
+            if (!(ok = mbar_wait_warp(&bars->o_full[t], no & 1, ctx))) break;
+            ++no;
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t a[32];
+              tmem_ld32(tO + q * 32, a);
+              tmem_wait_ld();
+              if (row_valid) {
+                float4* to = reinterpret_cast<float4*>(p.parts.o_accum + part_row * D + q * 32);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  to[i] = make_float4(__uint_as_float(a[4 * i]) * inv, __uint_as_float(a[4 * i + 1]) * inv,
+                                      __uint_as_float(a[4 * i + 2]) * inv, __uint_as_float(a[4 * i + 3]) * inv);
+              }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->o_read);
+          }
+          g += nb_max;
+          __syncwarp();
+          if (lane == 0) release_item(n);
+          continue;
         }
         if (row_valid) p.lse[(static_cast<int64_t>(w.batch) * 2 * p.h + 2 * w.head + t) * p.lse_row_stride + row] = lse_val;
         const int col0 = t * (D / 2);
@@ -883,7 +925,7 @@ int launch_items(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_
   kp.items_x = (seqlen_q + kItemRows - 1) / kItemRows;
   kp.b = b;
   const int64_t total = kp.cu_seqlens_q ? static_cast<int64_t>(h) * (total_q / (kDiff ? kBlockM : kTiles * kBlockM) + b)
-                                        : static_cast<int64_t>(kp.items_x) * h * b;
+                                        : static_cast<int64_t>(kp.items_x) * h * b * (kDiff ? kp.parts.splits : 1);
   FA_CHECK_ARG(total < (1ll << 30), "fa_fwd: too many work items");
   kp.total_items = static_cast<int>(total);
   // with a CTA for every item the order is moot, and neighbours of equal length are 2 % slower (B5 S3904 H1 D64: 61 : 60 us)
@@ -915,7 +957,8 @@ int launch_fwd(FwdKernelParams& kp, int b, int h, int seqlen_q, int64_t total_q,
 
 namespace fa {
 
-int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap, bool checked, const FaDiffFwdParams* diff) {
+int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool overlap, bool checked, const FaDiffFwdParams* diff,
+            const DiffSplits* parts) {
   FA_CHECK_ARG(p != nullptr, "fa_fwd: params is NULL");
   FA_CHECK_ARG(p->q && p->k && p->v && p->o && p->lse, "fa_fwd: q, k, v, o, lse must be non-NULL");
   if (p->d != 64 && p->d != 128)
@@ -1001,6 +1044,7 @@ int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool o
   kp.o2_batch_stride = diff ? diff->o2_batch_stride : 0;
   kp.o2_row_stride = diff ? diff->o2_row_stride : 0;
   kp.o2_head_stride = diff ? diff->o2_head_stride : 0;
+  kp.parts = parts ? *parts : DiffSplits{};
   kp.status = device_status_ptr();
   if (p->flags == FA_FWD_ZERO_UNUSED_ROWS && varlen_q) {  // no other value: see the header
     const PackedRows rows{kp.o, kp.o_row_stride, kp.o_head_stride, p->total_q, p->h, p->d, p->cu_seqlens_q, p->b};

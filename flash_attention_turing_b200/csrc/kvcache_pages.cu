@@ -323,6 +323,18 @@ struct MoveParams {
   const int* num_live;
 };
 
+// `bytes` of a page, kUnroll 16-byte units of a thread at a time, of which the first begins at `at`
+template <int kUnroll>
+__device__ __forceinline__ void copy_chunk(const uint8_t* src, uint8_t* dst, int64_t at, int64_t bytes) {
+  uint4 x[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i)
+    if (at + i * kCopyThreads * 16 < bytes) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + at + i * kCopyThreads * 16));
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i)
+    if (at + i * kCopyThreads * 16 < bytes) __stcs(reinterpret_cast<uint4*>(dst + at + i * kCopyThreads * 16), x[i]);
+}
+
 // kUnroll 16-byte units of a thread in flight: a chunk is kUnroll * 4 KB of a page of one cache
 template <int kUnroll>
 __global__ void __launch_bounds__(kCopyThreads) move_kernel(const __grid_constant__ MoveParams p) {
@@ -333,16 +345,8 @@ __global__ void __launch_bounds__(kCopyThreads) move_kernel(const __grid_constan
     const int64_t m = item / per_move;
     const int rest = static_cast<int>(item - m * per_move), cache = rest / p.chunks, chunk = rest - cache * p.chunks;
     const PageMove move = p.moves[m];
-    const int64_t at = static_cast<int64_t>(chunk) * kChunk + threadIdx.x * 16;
-    const uint8_t* src = p.base[cache] + move.src * p.page_stride[cache] + at;
-    uint8_t* dst = p.base[cache] + move.dst * p.page_stride[cache] + at;
-    uint4 x[kUnroll];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (at + i * kCopyThreads * 16 < move.bytes) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + i * kCopyThreads * 16));
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (at + i * kCopyThreads * 16 < move.bytes) __stcs(reinterpret_cast<uint4*>(dst + i * kCopyThreads * 16), x[i]);
+    copy_chunk<kUnroll>(p.base[cache] + move.src * p.page_stride[cache], p.base[cache] + move.dst * p.page_stride[cache],
+                        static_cast<int64_t>(chunk) * kChunk + threadIdx.x * 16, move.bytes);
   }
   if (p.to != nullptr) {
     const int live = *p.num_live, pages = p.t.num_pages;
@@ -354,6 +358,38 @@ __global__ void __launch_bounds__(kCopyThreads) move_kernel(const __grid_constan
       const int page = *entry;
       if (page >= live && page < pages) *entry = p.to[page];
     }
+  }
+}
+
+// Few pages (kFewPages at most): the plan of an entry is a look at all entries, which each CTA takes by itself, and no launch or
+// scratch memory is needed for it.  3 pages of 4 caches (768 KB) 9.4 -> 6.6 us a call, most of it the host's.
+constexpr int kFewPages = 512;
+struct FewParams {
+  uint8_t* base[kMaxCaches];
+  int64_t page_stride[kMaxCaches];
+  int64_t page_bytes;
+  const int *src, *dst;
+  uint8_t* done;
+  int caches, chunks, n, num_pages;
+};
+template <int kUnroll>
+__global__ void __launch_bounds__(kCopyThreads) copy_few_kernel(const __grid_constant__ FewParams p) {
+  constexpr int kChunk = kUnroll * kCopyThreads * 16;
+  const int per_entry = p.caches * p.chunks;
+  for (int item = blockIdx.x; item < p.n * per_entry; item += gridDim.x) {
+    const int i = item / per_entry, rest = item - i * per_entry, cache = rest / p.chunks, chunk = rest - cache * p.chunks;
+    const int src = p.src[i], dst = p.dst[i];
+    auto inside = [&](int page) { return page >= 0 && page < p.num_pages; };
+    bool bad = !inside(src) || !inside(dst);
+    for (int j = threadIdx.x; j < p.n; j += kCopyThreads) {
+      const int a = p.src[j], b = p.dst[j];
+      if (inside(a) && inside(b) && a != b) bad |= b == src || (src != dst && b == dst && j > i);
+    }
+    bad = __syncthreads_or(bad);
+    if (rest == 0 && threadIdx.x == 0) p.done[i] = !bad;
+    if (bad || src == dst) continue;
+    copy_chunk<kUnroll>(p.base[cache] + src * p.page_stride[cache], p.base[cache] + dst * p.page_stride[cache],
+                        static_cast<int64_t>(chunk) * kChunk + threadIdx.x * 16, p.page_bytes);
   }
 }
 
@@ -394,6 +430,25 @@ int check_workspace(const void* ws, size_t bytes, size_t need, const char* who) 
   return FA_OK;
 }
 
+// Chunks (16-byte units of a thread) as large as still give every SM some: a thread then has that many loads in flight
+int chunk_units(int64_t bytes, int sms) { return bytes >= sms * (8ll << 15) ? 8 : bytes >= sms * (4ll << 13) ? 2 : 1; }
+
+int launch_few(const FaPageCaches* c, int num_pages, const int* src, const int* dst, int n, uint8_t* done, cudaStream_t stream) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return set_error(FA_ERR_CUDA, "fa_pages_copy: device attributes not available");
+  FewParams p = {};
+  for (int i = 0; i < c->count; ++i) p.base[i] = static_cast<uint8_t*>(c->base[i]), p.page_stride[i] = c->page_stride[i];
+  p.page_bytes = c->page_bytes, p.src = src, p.dst = dst, p.done = done, p.caches = c->count, p.n = n, p.num_pages = num_pages;
+  const int units = chunk_units(static_cast<int64_t>(n) * c->count * c->page_bytes, sms);
+  const int64_t chunk = units * kCopyThreads * 16;
+  p.chunks = static_cast<int>((c->page_bytes + chunk - 1) / chunk);
+  const int64_t items = static_cast<int64_t>(n) * c->count * p.chunks;
+  const auto kernel = units == 8 ? copy_few_kernel<8> : units == 2 ? copy_few_kernel<2> : copy_few_kernel<1>;
+  kernel<<<static_cast<unsigned>(std::min<int64_t>(items, sms * 8)), kCopyThreads, 0, stream>>>(p);
+  FA_CHECK_CUDA(cudaGetLastError());
+  return FA_OK;
+}
+
 // most: moves that there can be
 int launch_moves(const FaPageCaches* c, const PageMove* moves, const int* count, int64_t most, const FaPageTables* t, const int* to,
                  const int* num_live, cudaStream_t stream) {
@@ -406,9 +461,7 @@ int launch_moves(const FaPageCaches* c, const PageMove* moves, const int* count,
       p.base[i] = static_cast<uint8_t*>(c->base[first + i]), p.page_stride[i] = c->page_stride[first + i];
     p.moves = moves, p.count = count;
     if (first + kMaxCaches >= c->count && t != nullptr) p.t = *t, p.to = to, p.num_live = num_live;  // the last launch
-    // Chunks as large as still give every SM some: a thread then has that many loads in flight
-    const int64_t bytes = most * p.caches * c->page_bytes;
-    const int unroll = bytes >= sms * (8ll << 15) ? 8 : bytes >= sms * (4ll << 13) ? 2 : 1;
+    const int unroll = chunk_units(most * p.caches * c->page_bytes, sms);
     const int64_t chunk = unroll * kCopyThreads * 16;
     p.chunks = static_cast<int>((c->page_bytes + chunk - 1) / chunk);
     const int64_t items = std::max<int64_t>(most * p.caches * p.chunks, 1);
@@ -422,6 +475,10 @@ int launch_moves(const FaPageCaches* c, const PageMove* moves, const int* count,
     }
   }
   return FA_OK;
+}
+
+bool copies_few(const FaPageCaches* c, int n) {  // the items are counted in 32 bits
+  return n <= kFewPages && c->count <= kMaxCaches && static_cast<int64_t>(n) * c->count * (c->page_bytes / 4096 + 1) < (1 << 30);
 }
 
 size_t workspace_bytes(int64_t rows, int64_t pages, int64_t entries) {
@@ -439,6 +496,11 @@ size_t workspace_bytes(int64_t rows, int64_t pages, int64_t entries) {
 extern "C" size_t fa_pages_workspace_bytes(int32_t rows, int32_t num_pages, int32_t entries) {
   if (rows < 0 || num_pages < 0 || entries < 0) return 0;
   return fa::workspace_bytes(rows, num_pages, entries);
+}
+
+extern "C" size_t fa_pages_copy_workspace_bytes(const FaPageCaches* caches, int32_t num_pages, int32_t n) {
+  if (caches == nullptr || num_pages < 0 || n < 0 || fa::copies_few(caches, n)) return 0;
+  return fa::workspace_bytes(0, num_pages, n);
 }
 
 extern "C" int fa_pages_reserve(const FaPageTables* t, const int32_t* new_tokens, int32_t new_tokens_all, int32_t page_size, uint8_t* granted,
@@ -525,6 +587,10 @@ extern "C" int fa_pages_copy(const FaPageCaches* caches, int32_t num_pages, cons
   FA_CHECK_ARG(n >= 0 && num_pages >= 1, "fa_pages_copy: n is negative or num_pages not positive");
   if (n == 0) return FA_OK;
   FA_CHECK_ARG(src && dst && done, "fa_pages_copy: src, dst, done must be non-NULL");
+  if (copies_few(caches, n)) {
+    rc = check_device_sm100();
+    return rc != FA_OK ? rc : launch_few(caches, num_pages, src, dst, n, done, stream);
+  }
   rc = check_workspace(workspace, bytes, workspace_bytes(0, num_pages, n), "fa_pages_copy");
   if (rc == FA_OK) rc = check_device_sm100();
   if (rc != FA_OK) return rc;

@@ -1159,9 +1159,33 @@ struct Plan {
   size_t lse = 0;         // scratch memory: offset of the LSE of the parts behind the parts, and the size
   size_t bytes = 0;
 };
+// Parts of the keys in the tiled kernel of differential calls: where two or more for each row tile find an SM, of at least kLeastChunk
+// blocks and one round at full capacity.  With more row tiles a second round, the partial rows and their merge cost more than the
+// longest sequence: 4 x 500-4000 tokens, 256 new ones, H16 (128 tiles) 61 us whole and 90 in chunks of 15 blocks.  One sequence of 16384
+// tokens: 64 new ones, H8 222 -> 34 us, 512 new ones 216 -> 79; 2 x 8192, 128 new ones, H16 D64 113 -> 47.
+constexpr int kTiledRows = 128, kTiledKeys = 128, kLeastChunk = 8;
+void plan_tiled_parts(const FaKvcacheParams* p, int* splits, int* chunk) {
+  const int64_t blocks = std::max<int64_t>(1, (static_cast<int64_t>(capacity_tokens(p)) + kTiledKeys - 1) / kTiledKeys);
+  const int64_t tiles = static_cast<int64_t>((p->seqlen_q + kTiledRows - 1) / kTiledRows) * (p->h / 2) * p->b;
+  const int64_t parts = std::min<int64_t>(64, p->num_splits > 0 ? p->num_splits : std::max<int64_t>(1, 148 / tiles));
+  int64_t each = (blocks + parts - 1) / parts;
+  if (p->num_splits == 0) each = std::max<int64_t>(each, kLeastChunk);
+  *splits = static_cast<int>((blocks + each - 1) / each);
+  *chunk = static_cast<int>(each);
+}
 Plan plan_call(const FaKvcacheParams* p, bool diff = false) {
   Plan plan;
-  if (!uses_decode_kernel(p, diff)) return plan;
+  if (!uses_decode_kernel(p, diff)) {
+    if (diff) {
+      plan_tiled_parts(p, &plan.splits, &plan.chunk);
+      if (plan.splits > 1) {
+        const size_t rows = static_cast<size_t>(plan.splits) * p->b * p->h * p->seqlen_q;
+        plan.lse = align_up(rows * p->d * sizeof(float), 256);
+        plan.bytes = plan.lse + align_up(rows * sizeof(float), 256);
+      }
+    }
+    return plan;
+  }
   if (p->num_splits > 0) {
     plan.splits = std::min(p->num_splits, 256);
   } else {
@@ -1334,8 +1358,16 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
     f.block_table_batch_stride = p->block_table_batch_stride;
     f.page_size = p->block_table ? p->seqlen_cache : 0;
     f.block_table_cols = p->block_table ? p->max_blocks_per_seq : 0;
-    if (diff) tiled.weights = *weights;
-    return run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr, diff ? &tiled : nullptr);
+    if (!diff) return run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr);
+    tiled.weights = *weights;
+    if (plan.splits == 1) return run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr, &tiled);
+    DiffSplits parts;
+    parts.splits = plan.splits, parts.chunk = plan.chunk, parts.rows = static_cast<int64_t>(p->b) * p->h * p->seqlen_q;
+    parts.o_accum = reinterpret_cast<float*>(scratch), parts.lse_accum = reinterpret_cast<float*>(scratch + plan.lse);
+    rc = run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr, &tiled, &parts);
+    if (rc != FA_OK) return rc;
+    return launch_diff_combine(parts.o_accum, parts.lse_accum, p->o, p->lse, parts.rows, plan.splits, p->h, p->seqlen_q, p->d,
+                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, stream);
   }
 
   const int64_t rows_total = static_cast<int64_t>(p->b) * p->h * p->seqlen_q;

@@ -156,9 +156,10 @@ at::Tensor pages_copy(std::vector<at::Tensor> caches, at::Tensor src, at::Tensor
   if (src.numel() == 0) return done;
   if (c.empty()) return done.zero_();
   const int32_t n = static_cast<int32_t>(src.numel());
-  at::Tensor ws = scratch(fa_pages_workspace_bytes(0, static_cast<int32_t>(c.pages), n), src);
-  check_rc(fa_pages_copy(&c.c, static_cast<int32_t>(c.pages), src.data_ptr<int>(), dst.data_ptr<int>(), n, flag_ptr(done), ws.data_ptr(),
-                         ws.numel(), current_stream()),
+  const size_t bytes = fa_pages_copy_workspace_bytes(&c.c, static_cast<int32_t>(c.pages), n);
+  at::Tensor ws = bytes > 0 ? scratch(bytes, src) : at::Tensor();
+  check_rc(fa_pages_copy(&c.c, static_cast<int32_t>(c.pages), src.data_ptr<int>(), dst.data_ptr<int>(), n, flag_ptr(done),
+                         bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
            "fa_pages_copy");
   return done;
 }

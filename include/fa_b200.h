@@ -448,7 +448,9 @@ int fa_pages_compact(const FaPageTables* t, const FaPageCaches* caches, int32_t*
                      fa_stream_t stream);
 
 /* Page dst[i] becomes a copy of page src[i] in every cache.  done[i] = 0, and nothing is copied: a page out of range, a         */
-/* destination that a later entry has too, a source that is the destination of another entry.                            */
+/* destination that a later entry has too, a source that is the destination of another entry.  Scratch:                    */
+/* fa_pages_copy_workspace_bytes() bytes, 0 for up to 512 entries and 128 caches.                                        */
+size_t fa_pages_copy_workspace_bytes(const FaPageCaches* caches, int32_t num_pages, int32_t n);
 int fa_pages_copy(const FaPageCaches* caches, int32_t num_pages, const int32_t* src, const int32_t* dst, int32_t n, uint8_t* done,
                   void* workspace, size_t workspace_bytes, fa_stream_t stream);
 

@@ -199,6 +199,9 @@ CACHE = [  # b, new, q rows, lengths, h, hk, d, page (0: contiguous), num_splits
     (2, 8, 8, [700, 1], 8, 2, 64, 256, 1),        # 64 rows, one split
     (2, 9, 9, [700, 1], 8, 2, 64, 256, 0),        # 72 rows: the tiled kernel
     (1, 4, 4, [50000], 2, 1, 128, 0, 0),          # a long cache, shared out over many CTAs
+    (1, 70, 70, [9000], 4, 2, 128, 256, 0),       # few row tiles, a long cache: its keys in parts
+    (3, 140, 140, [5, 2500, 0], 4, 1, 64, 0, 3),  # parts that some rows have no key in
+    (2, 100, 100, [1000, 3000], 8, 4, 64, 256, 1),
     (64, 1, 1, list(range(5, 645, 10)), 4, 2, 64, 256, 0),
     (40, 1, 1, list(range(100, 4100, 100)), 8, 4, 128, 256, 0),
 ]
