@@ -2,15 +2,18 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "common.h"
 
 namespace fa {
 
-inline int check_weights(const FaDiffWeights& w, int h, const char* who) {
+inline int check_weights(const FaDiffWeights& w, int h, float softmax_scale, const char* who) {
   FA_CHECK_ARG(w.lam != nullptr, std::string(who) + ": lam must be non-NULL");
   FA_CHECK_ARG(w.count == 1 || w.count == h, std::string(who) + ": weights.count must be 1 or h");
   FA_CHECK_ARG(w.is_half == 0 || w.is_half == 1, std::string(who) + ": weights.is_half must be 0 or 1");
+  // the row maximum is that of the unscaled scores, and the backward divides by the scale
+  FA_CHECK_ARG(softmax_scale >= 1e-6f && softmax_scale < INFINITY, std::string(who) + ": softmax_scale must be at least 1e-6");
   return FA_OK;
 }
 

@@ -22,16 +22,37 @@
 namespace fa {
 namespace {
 
-constexpr int kStatRows = 64;  // statistics of 64 rows lie together: -LSE_1, -LSE_2 (base 2), -delta_1, -delta_2, 64 floats each
-constexpr int kStatFloats = 4 * kStatRows;
+// Statistics of 64 rows lie together, 64 floats each: -LSE_1, -LSE_2 (base 2), -delta_1, -delta_2 (dQ kernel), delta_1 - delta_2 (dK/dV
+// kernel).  The dK/dV kernel, whose threads hold keys, would have to read the statistics of every query from shared memory, a wavefront for
+// each four bytes and warp: with the operands of the products that was 91 % of what the memory can deliver, 2470 clocks a tile.  There
+// the products add them: a 64-column row per query holds -LSE_1 / c, -LSE_2 / c and -delta_1 (c = scale * log2(e)), each cut into three fp16
+// numbers for three columns of a K = 16 slice of its own, whose other operand is the constants kSplit in every row.  So S_m comes
+// as S_m - LSE_m / c and dP as dP - delta_1.
+constexpr int kStatRows = 64;
+constexpr int kStatFloats = 5 * kStatRows;
+constexpr int kExtColumns = 64;  // slices at columns 0 (S_1), 16 (S_2), 32 (dP); 48-63 are not used
+// 2^15, 2^4, 2^-8: each number holds what the one before leaves over, 2^9 to 2^11 times smaller.  Up to 2 * 10^9 in all, the rest below
+// 2^-33 of the value (or 2^-32).
+__device__ __forceinline__ void split3(float x, __half (&h)[3]) {
+  h[0] = __float2half_rn(x * 0x1p-15f);
+  if (x == -INFINITY) {  // rows that do not exist
+    h[1] = h[2] = __float2half_rn(0.f);
+    return;
+  }
+  x -= __half2float(h[0]) * 0x1p15f;
+  h[1] = __float2half_rn(x * 0x1p-4f);
+  x -= __half2float(h[1]) * 0x1p4f;
+  h[2] = __float2half_rn(x * 0x1p8f);
+}
 
 struct DiffKernelParams {
   CUtensorMap tm_q, tm_k, tm_v, tm_do;  // boxes of 128 rows; dK/dV kernel: q and do of 64
+  CUtensorMap tm_ext;  // dK/dV kernel: (b * h * sq_pad, 64) fp16, boxes of 64 rows
   __half *dq, *dk, *dv;
   int64_t dq_batch_stride, dq_row_stride, dq_head_stride;
   int64_t dk_batch_stride, dk_row_stride, dk_head_stride;
   int64_t dv_batch_stride, dv_row_stride, dv_head_stride;
-  const float* stats;  // (b, h, sq_pad / 64, 4, 64)
+  const float* stats;  // (b, h, sq_pad / 64, 5, 64)
   int sq_pad;
   int seqlen_q, seqlen_k, h, h_k, group, b;
   float scale, scale_log2;
@@ -53,6 +74,8 @@ struct DiffPreParams {
   const __half *o, *o2, *dout;
   const float* lse;
   float* stats;
+  __half* ext;
+  float inv_scale_log2;  // 1 / c
   int64_t o_batch_stride, o_row_stride, o_head_stride;
   int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
   int64_t do_batch_stride, do_row_stride, do_head_stride;
@@ -113,7 +136,7 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
     float lse = 0.f;
     if (map < 2 && row0 + mine < sq) lse = p.lse[(2 * bh + map) * p.lse_row_stride + row0 + mine];
     const float lam = weight_of(p.weights, head);
-    float delta = 0.f;
+    float delta = 0.f, other = 0.f;  // of this lane's map, of the other one
 #pragma unroll
     for (int i = 0; i < kPreRows; ++i) {
       float x = dot8(a[i], c[i]), y = dot8(b[i], c[i]);
@@ -121,14 +144,31 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
         x += __shfl_xor_sync(0xffffffffu, x, off);
         y += __shfl_xor_sync(0xffffffffu, y, off);
       }
-      if (i == mine) delta = map == 0 ? fmaf(lam, y, x) : y;  // dO . A_1 V = dO . O + lam dO . A_2 V
+      if (i == mine) {  // dO . A_1 V = dO . O + lam dO . A_2 V
+        const float first = fmaf(lam, y, x);
+        delta = map == 0 ? first : y, other = map == 0 ? y : first;
+      }
     }
     if (map < 2 && row0 + mine < p.sq_pad) {
       const int row = row0 + mine;
       float* to = p.stats + (bh * (p.sq_pad / kStatRows) + row / kStatRows) * kStatFloats + row % kStatRows;
       const bool valid = row < sq;
-      to[map * kStatRows] = valid ? -lse * kLog2e : -INFINITY;
+      const float nl = valid ? -lse * kLog2e : -INFINITY;
+      to[map * kStatRows] = nl;
       to[(2 + map) * kStatRows] = valid ? -delta : 0.f;
+      if (map == 0) to[4 * kStatRows] = valid ? delta - other : 0.f;
+      // 16 columns of S_m, by the lane of map 1 those of dP too
+      uint4* ext = reinterpret_cast<uint4*>(p.ext + (bh * p.sq_pad + row) * kExtColumns);
+      auto put = [&](int slice, float x) {
+        __half h[4];
+        split3(x, reinterpret_cast<__half(&)[3]>(h));
+        h[3] = __float2half_rn(0.f);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(h);
+        ext[2 * slice] = make_uint4(w[0], w[1], 0u, 0u);
+        ext[2 * slice + 1] = make_uint4(0u, 0u, 0u, 0u);
+      };
+      put(map, nl * p.inv_scale_log2);
+      if (map == 0) put(2, valid ? -delta : 0.f);
     }
   }
   if constexpr (kClear) {  // the other kernels write all other rows of dq, dk, dv
@@ -239,6 +279,7 @@ constexpr int kDiffReaders = kComputeWarps + 2;  // elementwise warps, producer 
 constexpr int kDqSlots = 3;     // the item to be stored, the current one, the next (see the plain dQ kernel)
 constexpr int kDqKStages = 3;   // a K tile lives from S_1 of its block to dQ_2, which is issued a block later
 constexpr int kDqVStages = 2;
+constexpr int kDqStatFloats = 4 * kStatRows;  // without the last ones
 
 struct __align__(16) DiffDqItem {
   int nb;  // key blocks to visit; < 0: no more work
@@ -270,7 +311,7 @@ struct DqCfg {
   static constexpr int kChunkBytes = 128 * 128;
   static constexpr int kTileBytes = kChunks * kChunkBytes;
   static constexpr int kAlignPad = D == 128 ? 0 : 1024;  // no room: the kernel checks that its memory starts on 1024 bytes
-  static constexpr int kSmemBytes = (2 + kDqKStages + kDqVStages) * kTileBytes + 2 * kStatFloats * 4 + 1024 + kAlignPad;
+  static constexpr int kSmemBytes = (2 + kDqKStages + kDqVStages) * kTileBytes + 2 * kDqStatFloats * 4 + 1024 + kAlignPad;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -311,7 +352,7 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
   uint8_t* sK = sdO + C::kTileBytes;
   uint8_t* sV = sK + kDqKStages * C::kTileBytes;
   float* sStats = reinterpret_cast<float*>(sV + kDqVStages * C::kTileBytes);  // [row / 64][4][64]
-  DiffDqBarriers* bars = reinterpret_cast<DiffDqBarriers*>(sStats + 2 * kStatFloats);
+  DiffDqBarriers* bars = reinterpret_cast<DiffDqBarriers*>(sStats + 2 * kDqStatFloats);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kS1 = 0, kS2 = 128, kDP = 256, kAcc = 384;
 
@@ -417,14 +458,16 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
       if (lane == 0) {
         ok = mbar_wait(&bars->q_free, (ni & 1) ^ 1, ctx);
         if (ok) {
-          mbar_arrive_expect_tx(&bars->q_full, 2 * C::kTileBytes + 2 * kStatFloats * 4);
+          mbar_arrive_expect_tx(&bars->q_full, 2 * C::kTileBytes + 2 * kDqStatFloats * 4);
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c) {
             tma_load_4d(sQ + c * C::kChunkBytes, &p.tm_q, &bars->q_full, c * 64, w.head, w.q_off + w.row0, w.bq);
             tma_load_4d(sdO + c * C::kChunkBytes, &p.tm_do, &bars->q_full, c * 64, w.head, w.q_off + w.row0, w.bq);
           }
           const int64_t tile = (static_cast<int64_t>(w.batch) * p.h + w.head) * (p.sq_pad / kStatRows) + w.row0 / kStatRows;
-          bulk_load_1d(sStats, p.stats + tile * kStatFloats, 2 * kStatFloats * 4, &bars->q_full);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            bulk_load_1d(sStats + i * kDqStatFloats, p.stats + (tile + i) * kStatFloats, kDqStatFloats * 4, &bars->q_full);
         }
         for (int j = 0; ok && j < w.nb; ++j) {
           const int g = G + j, s = g % kDqKStages, sv = g % kDqVStages;
@@ -519,7 +562,7 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
     const int cq = warp >> 2, quarter = warp & 3;
     const int row_in_tile = quarter * 32 + lane;
     const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cq * 32;
-    const float* stats = sStats + row_in_tile / kStatRows * kStatFloats + row_in_tile % kStatRows;
+    const float* stats = sStats + row_in_tile / kStatRows * kDqStatFloats + row_in_tile % kStatRows;
     const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
     int G = 0, ni = 0, pending = -1;  // pending: the item whose dQ is still to be stored
     bool ok = true;
@@ -672,9 +715,10 @@ struct DkvCfg {
   static constexpr int kChunks = D / 64;
   static constexpr int kKvChunkBytes = 128 * 128, kKvTileBytes = kChunks * kKvChunkBytes;
   static constexpr int kQChunkBytes = kQRows * 128, kQTileBytes = kChunks * kQChunkBytes;
-  static constexpr int kStatBytes = kStatFloats * 4;
-  static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr int kSmemBytes = 2 * kKvTileBytes + kStages * (2 * kQTileBytes + kStatBytes) + 512 + 1024 /*alignment*/;
+  static constexpr int kExtBytes = kQRows * 128, kOnesBytes = 1024, kStatBytes = kStatRows * 4;
+  static constexpr int kStages = D == 128 ? 4 : 7;
+  static constexpr int kAlignPad = D == 128 ? 0 : 1024;  // no room: the kernel checks that its memory starts on 1024 bytes
+  static constexpr int kSmemBytes = 2 * kKvTileBytes + kOnesBytes + kStages * (2 * kQTileBytes + kExtBytes + kStatBytes) + 512 + kAlignPad;
   static_assert(kSmemBytes <= 227 * 1024 && kStages <= kMaxQStages, "shared memory budget");
 };
 
@@ -712,15 +756,22 @@ __device__ __forceinline__ void zero_q_rows_from(uint8_t* tile, int first_row, i
 template <int D, bool kVarlen>
 __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid_constant__ DiffKernelParams p) {
   using C = DkvCfg<D>;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int stop_probe = stop_probe_begin(p.status);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  if (smem - smem_raw > C::kAlignPad) {  // uniform over the CTA: nothing has been set up yet
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, kStatusSmemLayout);
+    grid_dependency_wait();
+    return;
+  }
   uint8_t* sK = smem;
   uint8_t* sV = sK + C::kKvTileBytes;
   uint8_t* sQ = sV + C::kKvTileBytes;
   uint8_t* sdO = sQ + C::kStages * C::kQTileBytes;
-  float* sStats = reinterpret_cast<float*>(sdO + C::kStages * C::kQTileBytes);
-  DiffDkvBarriers* bars = reinterpret_cast<DiffDkvBarriers*>(sStats + C::kStages * kStatFloats);
+  uint8_t* sExt = sdO + C::kStages * C::kQTileBytes;
+  uint8_t* sOnes = sExt + C::kStages * C::kExtBytes;  // eight rows of the constants of split3(), for all groups of eight keys
+  float* sStats = reinterpret_cast<float*>(sOnes + C::kOnesBytes);
+  DiffDkvBarriers* bars = reinterpret_cast<DiffDkvBarriers*>(sStats + C::kStages * kStatRows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kS1 = 0, kS2 = 64, kDP = 128, kP = 192, kDS1 = 224, kAccV = 256, kAccK = 256 + D;
 
@@ -748,6 +799,15 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
   if (warp == kMmaWarp) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
+  }
+  if (warp == 0) {
+    for (int u = lane; u < 64; u += 32) {  // 16-byte units of the eight rows; slices 0 to 2 begin at units 0, 2, 4
+      const int row = u >> 3, unit = u & 7;
+      const bool constants = (unit & 1) == 0 && unit < 6;
+      *reinterpret_cast<uint4*>(sOnes + row * 128 + ((unit ^ row) << 4)) =
+          constants ? make_uint4(pack_half2(0x1p15f, 0x1p4f), pack_half2(0x1p-8f, 0.f), 0u, 0u) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
   }
   tc_fence_before_sync();
   const bool stop = __syncthreads_or(stop_probe) != 0;
@@ -831,8 +891,9 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
         const int head = w.head_k * p.group + it / w.per_head, i = w.i_min + it % w.per_head;
         const int64_t tile = (static_cast<int64_t>(w.batch) * p.h + head) * (p.sq_pad / kStatRows) + i;
         if (!mbar_wait(&bars->q_empty[s], ((T / C::kStages) & 1) ^ 1, ctx)) return false;
-        mbar_arrive_expect_tx(&bars->q_full[s], 2 * C::kQTileBytes + C::kStatBytes);
-        bulk_load_1d(sStats + s * kStatFloats, p.stats + tile * kStatFloats, C::kStatBytes, &bars->q_full[s]);
+        mbar_arrive_expect_tx(&bars->q_full[s], 2 * C::kQTileBytes + C::kExtBytes + C::kStatBytes);
+        bulk_load_1d(sStats + s * kStatRows, p.stats + tile * kStatFloats + 4 * kStatRows, C::kStatBytes, &bars->q_full[s]);
+        tma_load_4d(sExt + s * C::kExtBytes, &p.tm_ext, &bars->q_full[s], 0, 0, static_cast<int>(tile) * kStatRows, 0);
 #pragma unroll
         for (int c = 0; c < C::kChunks; ++c) {
           tma_load_4d(sQ + s * C::kQTileBytes + c * C::kQChunkBytes, &p.tm_q, &bars->q_full[s], c * 64, head, w.q_off + i * kQRows, bq);
@@ -884,13 +945,21 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
       auto q_tile = [&](int T) { return smem_u32(sQ + (T % C::kStages) * C::kQTileBytes); };
       auto do_tile = [&](int T) { return smem_u32(sdO + (T % C::kStages) * C::kQTileBytes); };
       auto q_full = [&](int T) { return wait(&bars->q_full[T % C::kStages], (T / C::kStages) & 1); };
-      auto scores = [&](int T) {  // S_m^T = K_m Q_m^T
+      const uint64_t ones = make_smem_desc(smem_u32(sOnes), 16, 0);  // the same eight rows for every group of eight
+      auto statistics = [&](uint32_t d_tmem, int T, int slice) {  // their slice
+        const uint64_t ext = make_smem_desc(smem_u32(sExt + (T % C::kStages) * C::kExtBytes), 16, 1024);
+        mma_ss(d_tmem, desc_advance(ones, slice * 32), desc_advance(ext, slice * 32), idesc_s, 1u);
+      };
+      auto scores = [&](int T) {  // S_m^T = K_m Q_m^T - LSE_m / c
         product_slices<D, 128, kQRows>(tmem_base + kS1, k_addr, q_tile(T), idesc_s, 0, D / 32);
+        statistics(tmem_base + kS1, T, 0);
         product_slices<D, 128, kQRows>(tmem_base + kS2, k_addr, q_tile(T), idesc_s, D / 32, D / 32);
+        statistics(tmem_base + kS2, T, 1);
         tc_commit(&bars->s_full);
       };
-      auto dp = [&](int T) {  // dP^T = V dO^T
+      auto dp = [&](int T) {  // dP^T = V dO^T - delta_1
         product_slices<D, 128, kQRows>(tmem_base + kDP, v_addr, do_tile(T), idesc_s, 0, D / 16);
+        statistics(tmem_base + kDP, T, 2);
         tc_commit(&bars->dp_full);
       };
       int T0 = 0, ni = 0;
@@ -978,17 +1047,11 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
         tmem_ld16(t_base + kS2 + cq * 16, s2);
         tmem_wait_ld();
         warp_arrive_loaded(&bars->s_loaded, lane);  // the scores of the next tile may come
-        const float* stats = sStats + (T % C::kStages) * kStatFloats + cq * 16;
-        const float4* l1 = reinterpret_cast<const float4*>(stats);
-        const float4* l2 = reinterpret_cast<const float4*>(stats + kStatRows);
         float2 p1[8], p2[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 a = l1[e], b = l2[e];
-          p1[2 * e] = ffma2(make_float2(__uint_as_float(s1[4 * e]), __uint_as_float(s1[4 * e + 1])), c2, make_float2(a.x, a.y));
-          p1[2 * e + 1] = ffma2(make_float2(__uint_as_float(s1[4 * e + 2]), __uint_as_float(s1[4 * e + 3])), c2, make_float2(a.z, a.w));
-          p2[2 * e] = ffma2(make_float2(__uint_as_float(s2[4 * e]), __uint_as_float(s2[4 * e + 1])), c2, make_float2(b.x, b.y));
-          p2[2 * e + 1] = ffma2(make_float2(__uint_as_float(s2[4 * e + 2]), __uint_as_float(s2[4 * e + 3])), c2, make_float2(b.z, b.w));
+        for (int e = 0; e < 8; ++e) {
+          p1[e] = fmul2(make_float2(__uint_as_float(s1[2 * e]), __uint_as_float(s1[2 * e + 1])), c2);
+          p2[e] = fmul2(make_float2(__uint_as_float(s2[2 * e]), __uint_as_float(s2[2 * e + 1])), c2);
         }
         exp2_pairs(p1);
         exp2_pairs(p2);
@@ -1019,17 +1082,16 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
         uint32_t dp[16];
         tmem_ld16(t_base + kDP + cq * 16, dp);
         tmem_st8(t_base + kP + cq * 8, pk);
-        const float4* d1 = reinterpret_cast<const float4*>(stats + 2 * kStatRows);
-        const float4* d2 = reinterpret_cast<const float4*>(stats + 3 * kStatRows);
+        const float4* differences = reinterpret_cast<const float4*>(sStats + (T % C::kStages) * kStatRows + cq * 16);
         tmem_wait_ld();
         uint32_t pk2[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float4 a = d1[e], b = d2[e];
+          const float4 a = differences[e];
           const float2 x = make_float2(__uint_as_float(dp[4 * e]), __uint_as_float(dp[4 * e + 1]));
           const float2 y = make_float2(__uint_as_float(dp[4 * e + 2]), __uint_as_float(dp[4 * e + 3]));
-          const float2 u0 = fmul2(p1[2 * e], fadd2(x, make_float2(a.x, a.y))), u1 = fmul2(p1[2 * e + 1], fadd2(y, make_float2(a.z, a.w)));
-          const float2 v0 = fmul2(p2[2 * e], fadd2(x, make_float2(b.x, b.y))), v1 = fmul2(p2[2 * e + 1], fadd2(y, make_float2(b.z, b.w)));
+          const float2 u0 = fmul2(p1[2 * e], x), u1 = fmul2(p1[2 * e + 1], y);
+          const float2 v0 = fmul2(p2[2 * e], fadd2(x, make_float2(a.x, a.y))), v1 = fmul2(p2[2 * e + 1], fadd2(y, make_float2(a.z, a.w)));
           pk[2 * e] = pack_half2(u0.x, u0.y), pk[2 * e + 1] = pack_half2(u1.x, u1.y);
           pk2[2 * e] = pack_half2(v0.x, v0.y), pk2[2 * e + 1] = pack_half2(v1.x, v1.y);
         }
@@ -1095,8 +1157,9 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 size_t stats_bytes(const FaBwdParams& p) {
-  return align256(static_cast<size_t>(p.b) * p.h * round_up(p.seqlen_q, kBlock) * 4 * sizeof(float));
+  return align256(static_cast<size_t>(p.b) * p.h * round_up(p.seqlen_q, kBlock) / kStatRows * kStatFloats * sizeof(float));
 }
+size_t ext_bytes(const FaBwdParams& p) { return static_cast<size_t>(p.b) * p.h * round_up(p.seqlen_q, kBlock) * kExtColumns * sizeof(__half); }
 
 template <class Kernel>
 int configure(Kernel kernel, int smem, bool (&done)[64]) {
@@ -1150,7 +1213,7 @@ int launch(const FaBwdParams& b, DiffKernelParams kp, const CUtensorMap& q64, co
 extern "C" size_t fa_diff_bwd_workspace_bytes(const FaDiffBwdParams* p) {
   using namespace fa;
   if (p == nullptr || p->base.b < 1 || p->base.h < 1 || p->base.seqlen_q < 1) return 0;
-  return stats_bytes(p->base) + align256(static_cast<size_t>(p->base.h) * sizeof(float));
+  return stats_bytes(p->base) + ext_bytes(p->base) + align256(static_cast<size_t>(p->base.h) * sizeof(float));
 }
 
 extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
@@ -1167,7 +1230,7 @@ extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
   FA_CHECK_ARG(b.lse_row_stride >= b.seqlen_q, "fa_diff_bwd: lse_row_stride is smaller than seqlen_q");
   FA_CHECK_ARG(b.is_causal >= 0 && b.is_causal <= 2 && (b.is_causal != 2 || b.cu_seqlens_q == nullptr), "fa_diff_bwd: bad is_causal");
   FA_CHECK_ARG((b.flags & ~FA_BWD_ZERO_UNUSED_ROWS) == 0, "fa_diff_bwd: flags must be 0 or FA_BWD_ZERO_UNUSED_ROWS");
-  int rc = check_weights(p->weights, b.h, "fa_diff_bwd");
+  int rc = check_weights(p->weights, b.h, b.softmax_scale, "fa_diff_bwd");
   if (rc != FA_OK) return rc;
   const bool varlen = b.cu_seqlens_q != nullptr;
   {
@@ -1204,6 +1267,8 @@ extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
   pp.o = static_cast<const __half*>(b.o), pp.o2 = static_cast<const __half*>(p->o2), pp.dout = static_cast<const __half*>(b.dout);
   pp.lse = b.lse;
   pp.stats = static_cast<float*>(b.workspace);
+  pp.ext = reinterpret_cast<__half*>(static_cast<uint8_t*>(b.workspace) + stats_bytes(b));
+  pp.inv_scale_log2 = 1.f / (b.softmax_scale * kLog2e);
   pp.o_batch_stride = b.o_batch_stride, pp.o_row_stride = b.o_row_stride, pp.o_head_stride = b.o_head_stride;
   pp.o2_batch_stride = p->o2_batch_stride, pp.o2_row_stride = p->o2_row_stride, pp.o2_head_stride = p->o2_head_stride;
   pp.do_batch_stride = b.do_batch_stride, pp.do_row_stride = b.do_row_stride, pp.do_head_stride = b.do_head_stride;
@@ -1236,6 +1301,10 @@ extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
   kp.dk_batch_stride = b.dk_batch_stride, kp.dk_row_stride = b.dk_row_stride, kp.dk_head_stride = b.dk_head_stride;
   kp.dv_batch_stride = b.dv_batch_stride, kp.dv_row_stride = b.dv_row_stride, kp.dv_head_stride = b.dv_head_stride;
   kp.stats = pp.stats;
+  const int64_t ext_rows = static_cast<int64_t>(b.b) * b.h * pp.sq_pad;
+  FA_CHECK_ARG(ext_rows < (1ll << 31), "fa_diff_bwd: too many rows");
+  rc = make_tensor_map_4d(&kp.tm_ext, pp.ext, kExtColumns, 1, ext_rows, 1, kExtColumns, kExtColumns, 0, kQRows, "fa_diff_bwd: workspace");
+  if (rc != FA_OK) return rc;
   kp.sq_pad = pp.sq_pad;
   kp.seqlen_q = b.seqlen_q, kp.seqlen_k = b.seqlen_k, kp.h = b.h, kp.h_k = b.h_k, kp.group = b.h / b.h_k, kp.b = b.b;
   kp.scale = b.softmax_scale, kp.scale_log2 = b.softmax_scale * kLog2e;
@@ -1243,7 +1312,7 @@ extern "C" int fa_diff_bwd(const FaDiffBwdParams* p, fa_stream_t stream_) {
   kp.cu_seqlens_q = b.cu_seqlens_q, kp.cu_seqlens_k = b.cu_seqlens_k;
   kp.weights = p->weights;
   const bool joins = p->weights.count == 1 && b.h > 1;
-  kp.head_dlam = joins ? reinterpret_cast<float*>(static_cast<uint8_t*>(b.workspace) + stats_bytes(b)) : nullptr;
+  kp.head_dlam = joins ? reinterpret_cast<float*>(static_cast<uint8_t*>(b.workspace) + stats_bytes(b) + ext_bytes(b)) : nullptr;
   kp.dlam = p->dlam;
   kp.status = device_status_ptr();
   rc = b.d == 128 ? launch<128>(b, kp, q64, do64, stream) : launch<64>(b, kp, q64, do64, stream);

@@ -1074,7 +1074,7 @@ extern "C" int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream) {
   FA_CHECK_ARG(b.q && b.k && b.v && b.o && b.lse, "fa_diff_fwd: q, k, v, o, lse must be non-NULL");
   if (b.d != 64 && b.d != 128) return set_error(FA_ERR_UNSUPPORTED, "fa_diff_fwd: head_dim must be 64 or 128");
   FA_CHECK_ARG(b.b >= 1 && b.h >= 1 && b.h_k >= 1 && b.h % b.h_k == 0, "fa_diff_fwd: bad b / h / h_k");
-  const int rc = check_weights(p->weights, b.h, "fa_diff_fwd");
+  const int rc = check_weights(p->weights, b.h, b.softmax_scale, "fa_diff_fwd");
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(aligned16(p->o2) && p->o2_batch_stride % 8 == 0 && p->o2_row_stride % 8 == 0 && p->o2_head_stride % 8 == 0,
                "fa_diff_fwd: o2 must be 16-byte aligned with strides that are multiples of 8 elements");

@@ -1459,7 +1459,7 @@ extern "C" int fa_diff_kvcache(const FaDiffKvcacheParams* p, int32_t* verdict, i
   using namespace fa;
   FA_CHECK_ARG(p != nullptr, "fa_diff_kvcache: params is NULL");
   int rc = validate(&p->base, "fa_diff_kvcache");
-  if (rc == FA_OK) rc = check_weights(p->weights, p->base.h, "fa_diff_kvcache");
+  if (rc == FA_OK) rc = check_weights(p->weights, p->base.h, p->base.softmax_scale, "fa_diff_kvcache");
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(p->base.h < (1 << 30), "fa_diff_kvcache: too many heads");
   FA_CHECK_ARG(verdict == nullptr || (token >= 0 && token < (1 << 30)), "fa_diff_kvcache: token out of range");

@@ -8,7 +8,7 @@ Shapes, masks (bottom-right aligned), grouped heads, packed sequences and the KV
 ``flash_attn_varlen_func`` and ``flash_attn_with_kvcache``: fp16, head dimension 64 or 128 (maps of 32 or 64).  A model that keeps
 2 * nheads query heads of d / 2 and values of d passes ``q.view(b, s, nheads, d)``: the two maps of a head lie next to each other.
 ``lam`` holds one weight per query head, or a single one for all, fp32 or fp16, and has a gradient.  What a model puts around the
-operator (how lam is parametrised, a norm of the heads' outputs) is its own.
+operator (how lam is parametrised, a norm of the heads' outputs) is its own.  ``softmax_scale`` must be at least 1e-6.
 No counterpart in Cy-47/flash-attention-turing.
 """
 from __future__ import annotations
