@@ -327,6 +327,7 @@ __device__ __forceinline__ void make_dq_item(const DiffKernelParams& p, int batc
   w.head_k = head / p.group;
   const int nkb = (w.sk + kBlock - 1) / kBlock;
   w.shift = (p.is_causal == 2) ? p.causal_shift : w.sk - w.sq;
+  w.sq = min(w.sq, p.seqlen_q);  // rows past max_seqlen_q have no statistics
   w.nb = nkb;
   if (p.is_causal) {
     const int x = w.row0 + kBlock + w.shift;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
               head = at.head, mblk = (sq + kBlock - 1) / kBlock - 1 - at.place;
             }
           }
-          if (mblk >= 0 && mblk * kBlock < sq) {
+          if (mblk >= 0 && mblk * kBlock < min(sq, p.seqlen_q)) {
             make_dq_item(p, batch, head, mblk, it);
             break;
           }
@@ -729,9 +730,10 @@ __device__ __forceinline__ DiffDkvWork decode_dkv(const DiffKernelParams& p, con
   DiffDkvWork w;
   w.batch = it.batch, w.head_k = it.head_k, w.q_off = it.q_off, w.k_off = it.k_off, w.sq = it.sq, w.sk = it.sk;
   w.key0 = it.nblk * kBlock;
+  w.shift = (p.is_causal == 2) ? p.causal_shift : w.sk - w.sq;  // key j visible to query i iff j <= i + shift
+  w.sq = min(w.sq, p.seqlen_q);  // rows past max_seqlen_q have no statistics
   w.nq = (w.sq + kQRows - 1) / kQRows;
   w.i_min = 0;
-  w.shift = (p.is_causal == 2) ? p.causal_shift : w.sk - w.sq;  // key j visible to query i iff j <= i + shift
   if (p.is_causal) {
     const int first_row = w.key0 - w.shift;  // first query row that can see key0
     w.i_min = first_row <= 0 ? 0 : first_row / kQRows;

@@ -175,6 +175,7 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
   w.head_k = w.head / (D == 64 ? p.h / p.h_k : p.group);
   // causal diagonal: key j is visible to query i iff j <= i + shift
   w.shift = (p.is_causal == 2) ? p.causal_shift : w.sk - w.sq;
+  if (kDiff) w.sq = min(w.sq, p.seqlen_q);  // rows past max_seqlen_q have no place in the LSE
   if (kItemRows == kBlockM && !kDiff) w.sq = min(w.sq, w.row0 + kBlockM);  // the rows after the item's only tile are not its own
   // number of K/V blocks each tile visits
   w.nkb = (w.sk + kBlockN - 1) / kBlockN;
@@ -759,16 +760,14 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         if (p.o2 != nullptr)
           o2row = p.o2 + (varlen_q ? static_cast<int64_t>(w.q_off + row) * p.o2_row_stride
                                    : w.batch * p.o2_batch_stride + static_cast<int64_t>(row) * p.o2_row_stride) + w.head * p.o2_head_stride;
-        auto store = [&](__half* to, const uint32_t (&x)[32], int col) {
+        const int rows_left = w.sq - (row - lane);  // of the warp's rows, those that exist
+        // 32 columns of the warp's rows, through store_rows_fp16(): with a row per lane the stores of an item took 2400 clocks with A_2 V,
+        // which the next item's loads from shared memory had to wait for
+        auto store = [&](__half* row_at, int64_t row_stride, const uint32_t (&x)[32], int col) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 v;
-            v.x = pack_half2(__uint_as_float(x[8 * i + 0]), __uint_as_float(x[8 * i + 1]));
-            v.y = pack_half2(__uint_as_float(x[8 * i + 2]), __uint_as_float(x[8 * i + 3]));
-            v.z = pack_half2(__uint_as_float(x[8 * i + 4]), __uint_as_float(x[8 * i + 5]));
-            v.w = pack_half2(__uint_as_float(x[8 * i + 6]), __uint_as_float(x[8 * i + 7]));
-            *reinterpret_cast<uint4*>(to + col + i * 8) = v;
-          }
+          for (int i = 0; i < 16; ++i) pk[i] = pack_half2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+          store_rows_fp16(row_at - lane * row_stride + col, row_stride, rows_left, pk, lane);
         };
         if (nbt > 0) {
           float* mine = factors + (no & 1) * 2 * kBlockM + row_in_tile;
@@ -794,16 +793,14 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
               __syncwarp();
               if (lane == 0) mbar_arrive(&bars->o_read);
             }
-            if (row_valid) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                a[i] = inv1 == 0.f ? 0u : __float_as_uint(fmaf(__uint_as_float(b[i]), minus, __uint_as_float(a[i]) * inv1));
-              store(orow, a, col0 + q * 32);
-              if (o2row != nullptr) {
+            for (int i = 0; i < 32; ++i)
+              a[i] = inv1 == 0.f ? 0u : __float_as_uint(fmaf(__uint_as_float(b[i]), minus, __uint_as_float(a[i]) * inv1));
+            store(orow, p.o_row_stride, a, col0 + q * 32);
+            if (o2row != nullptr) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) b[i] = inv2 == 0.f ? 0u : __float_as_uint(__uint_as_float(b[i]) * inv2);
-                store(o2row, b, col0 + q * 32);
-              }
+              for (int i = 0; i < 32; ++i) b[i] = inv2 == 0.f ? 0u : __float_as_uint(__uint_as_float(b[i]) * inv2);
+              store(o2row, p.o2_row_stride, b, col0 + q * 32);
             }
           }
           ++no;

@@ -374,6 +374,53 @@ def test_parameter_and_the_class_behind_the_native_node():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_transforms_and_modes_go_to_the_class(packed):
+    """functorch transforms and forward-mode AD are refused, a mode and a tensor subclass reach the class; saved tensors are guarded."""
+    from torch.overrides import TorchFunctionMode
+
+    gen, module = _gen(16), fa.diff_attention_interface
+    shape = (40,) if packed else (1, 40)
+    inputs = [_randn(gen, *shape, 2, 64), _randn(gen, *shape, 2, 64), _randn(gen, *shape, 2, 64), _lam(gen, 2)]
+    cu = torch.tensor([0, 15, 40], dtype=torch.int32, device="cuda")
+    cls = module.FlashDiffAttnVarlenFunc if packed else module.FlashDiffAttnFunc
+
+    def call(*x):
+        return fa.flash_diff_attn_varlen_func(*x, cu, cu, 25, 25, causal=True) if packed else fa.flash_diff_attn_func(*x, causal=True)
+
+    with pytest.raises(RuntimeError, match="functorch transforms"):
+        torch.func.vmap(call)(*(x[None] for x in inputs))
+    with torch.autograd.forward_ad.dual_level():
+        for i in (0, 3):
+            dual = [torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate(inputs)]
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call(*dual)
+    want, applied, real = call(*inputs), [], cls.apply
+    try:
+        cls.apply = classmethod(lambda c, *a: applied.append(1) or real(*a))
+
+        class Mode(TorchFunctionMode):
+            def __torch_function__(self, func, types, args=(), kwargs=None):
+                return func(*args, **(kwargs or {}))
+
+        with Mode():
+            assert torch.equal(call(*inputs), want)
+        sub = call(inputs[0].as_subclass(type("Sub", (torch.Tensor,), {})), *inputs[1:])
+        assert torch.equal(sub.as_subclass(torch.Tensor), want) and len(applied) == 2
+    finally:
+        del cls.apply
+    leaves, dout = [x.clone().requires_grad_() for x in inputs], _randn(gen, *inputs[0].shape)
+    out = call(*leaves)
+    native = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    extra = (cu, cu, 25, 25) if packed else ()
+    by_class = torch.autograd.grad(cls.apply(*leaves, *extra, None, True, True), leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(native, by_class))
+    with torch.no_grad():
+        leaves[3].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, leaves, dout)
+
+
 def test_refusals():
     q, k, lam = torch.zeros(1, 4, 4, 64, device="cuda").half(), torch.zeros(1, 4, 2, 64, device="cuda").half(), torch.zeros(4, device="cuda")
     for args, text in (
@@ -389,6 +436,13 @@ def test_refusals():
     ):
         with pytest.raises(RuntimeError, match=text):
             fa.flash_diff_attn_func(*args)
+    for scale in (0.0, -0.1, float("nan")):
+        with pytest.raises(RuntimeError, match="softmax_scale"):
+            fa.flash_diff_attn_func(q, k, k, lam, softmax_scale=scale)
+        with pytest.raises(RuntimeError, match="softmax_scale"):
+            fa.flash_diff_attn_with_kvcache(q, k, k, lam, cache_seqlens=2, softmax_scale=scale)
+    with pytest.raises(RuntimeError, match="same number of rows"):
+        fa.flash_diff_attn_with_kvcache(q, k, k.expand(2, -1, -1, -1), lam, cache_seqlens=2)
     cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="int32"):
         fa.flash_diff_attn_varlen_func(q[0], k[0], k[0], lam, cu.long(), cu, 4, 4)

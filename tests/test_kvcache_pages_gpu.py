@@ -192,6 +192,22 @@ def test_random_serving_steps(rows, columns, pages, page, layers, heads, d, dtyp
         c.compare()
 
 
+@pytest.mark.parametrize("n", [512, 513, 2500])
+def test_copies_of_many_pages(n):
+    """Up to 512 entries are looked at by every CTA, more by a kernel of their own."""
+    rng, pages = random.Random(n), 3000
+    m = Model(1, 1, pages, 2)
+    m.data = [[p % 90] * 2 for p in range(pages)]
+    c = Cache(m, 1, 1, 8)
+    src, dst = ([rng.randrange(-1, pages + 1) for _ in range(n)] for _ in range(2))
+    assert fa.kvcache_copy_pages(c.caches, _int(src), _int(dst)).tolist() == m.copy(src, dst)
+    c.compare()
+    order = rng.sample(range(pages), pages)  # none in another's way
+    src, dst = order[:n // 2], order[-(n // 2):]
+    assert fa.kvcache_copy_pages(c.caches, _int(src), _int(dst)).all() and all(m.copy(src, dst))
+    c.compare()
+
+
 def test_rows_behind_one_that_cannot_be_served():
     m = Model(5, 8, 6, 32)
     c = Cache(m)
