@@ -7,8 +7,8 @@
 // as two query heads with half of d set to zero it took those of two.  What stays double is the exponentials.
 //
 //   1. preprocess   -delta_1, -delta_2 and -LSE_m * log2(e) per row, from dO, O, A_2 V; interleaved by 64 rows (one copy per tile)
-//   2. dQ kernel    items of 128 query rows, over blocks of 128 keys
-//   3. dK/dV kernel items of 128 keys of a KV head, over the 64-row Q tiles of the heads of its group
+//   2. dK/dV kernel items of 128 keys of a KV head, over the 64-row Q tiles of the heads of its group; beside it dlam
+//   3. dQ kernel    items of 128 query rows, over blocks of 128 keys
 // Both are persistent, with the warp roles, rings and work counters of the plain backward (bwd_sm100.cu): sixteen elementwise warps (four
 // threads per TMEM lane), a TMA producer, one thread that issues the products, a scheduler.  Every result is bitwise reproducible.
 #include "bwd_common.cuh"
@@ -68,7 +68,7 @@ struct DiffKernelParams {
 };
 
 // =============================================================================================
-// 1. preprocess
+// preprocess
 // =============================================================================================
 struct DiffPreParams {
   const __half *o, *o2, *dout;
@@ -267,14 +267,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 // =============================================================================================
-// 2. dQ kernel
+// dQ kernel
 // =============================================================================================
 // TMEM: S_1 [0, 128), S_2 [128, 256), dP [256, 384), dQ [384, 384 + D), all of it at D = 128.  A thread packs dS_m into the first 16 of
 // its own 32 columns of S_m, so that no other thread's scores are in the way; the dQ products take their slices from there.
 // The elementwise warps go through a block map by map, dP in registers: while they are at map 2, dQ_1 of the block and S_1, dP of the
 // next one run, while they are at map 1 of the next, dQ_2 and S_2.  Nothing is double-buffered and nothing stands still.
 constexpr int kDiffThreads = 608;
-constexpr int kDiffSched = 18;  // dQ kernel: then sums dlam
+constexpr int kDiffSched = 18;
 constexpr int kDiffReaders = kComputeWarps + 2;  // elementwise warps, producer warp, issuing thread
 constexpr int kDqSlots = 3;     // the item to be stored, the current one, the next (see the plain dQ kernel)
 constexpr int kDqKStages = 3;   // a K tile lives from S_1 of its block to dQ_2, which is issued a block later
@@ -376,9 +376,6 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
     mbar_init(&bars->sched_go, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
-    grid_dependency_wait();  // the row statistics; everything behind the synchronisation below may read them
-    fence_acq_rel_gpu();     // ... and so may the dK/dV kernel, which starts behind the next line without a wait of its own
-    grid_launch_dependents();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
@@ -443,9 +440,6 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
         }
       }
     }
-    __syncwarp();
-    // while the other roles are at the last items
-    for (int head = blockIdx.x; head < p.h; head += gridDim.x) sum_dlam(p, head, lane);
   } else if (warp == kProducerWarp) {
     int G = 0, ni = 0, nf = 0;
     for (int n = 0;; ++n) {
@@ -677,6 +671,8 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
     }
     __syncthreads();
   }
+  // the dK/dV kernel may still be running: this launch must not complete before it
+  if (blockIdx.x == 0 && threadIdx.x == 0) grid_dependency_wait();
   if (warp == kMmaWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kTmemCols);
@@ -684,7 +680,7 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
 }
 
 // =============================================================================================
-// 3. dK/dV kernel
+// dK/dV kernel
 // =============================================================================================
 // TMEM: S_1^T [0, 64), S_2^T [64, 128), dP^T [128, 192), packed P^T [192, 224) and dS_1^T [224, 256), dV [256, 256 + D), dK behind it; the
 // packed dS_2^T lies in the threads' own columns of dP^T.  Q tiles of 64 rows, because three score tiles of 128 columns do not fit beside the
@@ -693,6 +689,9 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
 // of the tile before are over, and with them their packed operands), P^T and dS_m^T written and handed over together; then dV, dK_1, dK_2
 // and dP^T of the next tile run under its exponentials.
 constexpr int kQRows = 64;
+constexpr int kDkvThreads = 640;
+constexpr int kLamWarp = 19;  // sums dlam of a head while the others work: at the end of a launch it would be waited for
+static_assert((kDkvThreads / 32 + 3) / 4 * 32 * 96 <= 16384, "register file of one SM sub-partition");
 
 struct __align__(16) DiffDkvItem {
   int batch, head_k, nblk, q_off;  // nblk < 0: no more work
@@ -756,7 +755,7 @@ __device__ __forceinline__ void zero_q_rows_from(uint8_t* tile, int first_row, i
 }
 
 template <int D, bool kVarlen>
-__global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid_constant__ DiffKernelParams p) {
+__global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_constant__ DiffKernelParams p) {
   using C = DkvCfg<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int stop_probe = stop_probe_begin(p.status);
@@ -797,6 +796,9 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
     mbar_init(&bars->sched_go, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
+    grid_dependency_wait();  // the row statistics; everything behind the synchronisation below may read them
+    fence_acq_rel_gpu();     // ... and so may the dQ kernel, which starts behind the next line without a wait of its own
+    grid_launch_dependents();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
@@ -824,6 +826,8 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
   auto release_item = [&](int n) { mbar_arrive(&bars->sched_empty[n & 1]); };
 
   if (stop) {
+  } else if (warp == kLamWarp) {
+    for (int head = blockIdx.x; head < p.h; head += gridDim.x) sum_dlam(p, head, lane);
   } else if (warp == kDiffSched) {
     if (lane == 0) {
       bool finished = false;
@@ -1148,8 +1152,6 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dkdv_kernel(const __grid
     }
     __syncthreads();
   }
-  // the dQ kernel may still be running: this launch must not complete before it
-  if (blockIdx.x == 0 && threadIdx.x == 0) grid_dependency_wait();
   if (warp == kMmaWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kTmemCols);
@@ -1176,17 +1178,19 @@ int configure(Kernel kernel, int smem, bool (&done)[64]) {
 
 // One launch of a persistent kernel
 template <class Kernel>
-int launch_persistent(Kernel kernel, DiffKernelParams kp, int64_t total, int smem, cudaStream_t stream) {
+int launch_persistent(Kernel kernel, DiffKernelParams kp, int64_t total, int threads, int smem, cudaStream_t stream) {
   const int sms = device_sm_count();
   kp.sched = next_sched_slot(stream);
   if (sms <= 0 || kp.sched == nullptr) return set_error(FA_ERR_CUDA, "fa_diff_bwd: device attributes not available");
   FA_CHECK_ARG(total < (1ll << 30), "fa_diff_bwd: too many work items");
   kp.total_items = static_cast<int>(total);
-  FA_CHECK_CUDA(launch_overlapped(kernel, dim3(std::min(kp.total_items, sms)), kDiffThreads, smem, stream, kp));
+  FA_CHECK_CUDA(launch_overlapped(kernel, dim3(std::min(kp.total_items, sms)), threads, smem, stream, kp));
   return FA_OK;
 }
 
-// The three kernels overlap as those of the plain backward do (see launch_bwd there)
+// The kernels overlap as those of the plain backward do, the other way round: the dK/dV kernel waits for the statistics and then lets the
+// dQ kernel start, which reads nothing that it writes, on the SMs that it leaves.  Its items are long ones (a key tile of a KV head times all
+// queries of the group), those of the dQ kernel short, and what is left at the end of the launch is a short one then.
 template <int D>
 int launch(const FaBwdParams& b, DiffKernelParams kp, const CUtensorMap& q64, const CUtensorMap& do64, cudaStream_t stream) {
   static bool dq_done[64] = {}, dense_done[64] = {}, varlen_done[64] = {};
@@ -1195,18 +1199,19 @@ int launch(const FaBwdParams& b, DiffKernelParams kp, const CUtensorMap& q64, co
   if (rc == FA_OK) rc = configure(diff_dkdv_kernel<D, true>, DkvCfg<D>::kSmemBytes, varlen_done);
   if (rc != FA_OK) return rc;
   const bool varlen = kp.cu_seqlens_q != nullptr;
+  DiffKernelParams kk = kp;
+  kk.tm_q = q64, kk.tm_do = do64;
+  kk.items_x = (b.seqlen_k + kBlock - 1) / kBlock;
+  kk.section_rows = section_rows(b.is_causal != 0, b.seqlen_q, b.seqlen_k, static_cast<int64_t>(4 * D) * kp.group);
+  rc = launch_persistent(varlen ? diff_dkdv_kernel<D, true> : diff_dkdv_kernel<D, false>, kk,
+                         varlen ? static_cast<int64_t>(b.h_k) * (b.total_k / kBlock + b.b) : static_cast<int64_t>(kk.items_x) * b.h_k * b.b,
+                         kDkvThreads, DkvCfg<D>::kSmemBytes, stream);
+  if (rc != FA_OK) return rc;
   kp.items_x = (b.seqlen_q + kBlock - 1) / kBlock;
   kp.section_rows = section_rows(b.is_causal != 0, b.seqlen_q, b.seqlen_k, 4 * D);
-  rc = launch_persistent(diff_dq_kernel<D>, kp,
-                         varlen ? static_cast<int64_t>(b.h) * (b.total_q / kBlock + b.b) : static_cast<int64_t>(kp.items_x) * b.h * b.b,
-                         DqCfg<D>::kSmemBytes, stream);
-  if (rc != FA_OK) return rc;
-  kp.tm_q = q64, kp.tm_do = do64;
-  kp.items_x = (b.seqlen_k + kBlock - 1) / kBlock;
-  kp.section_rows = section_rows(b.is_causal != 0, b.seqlen_q, b.seqlen_k, static_cast<int64_t>(4 * D) * kp.group);
-  return launch_persistent(varlen ? diff_dkdv_kernel<D, true> : diff_dkdv_kernel<D, false>, kp,
-                           varlen ? static_cast<int64_t>(b.h_k) * (b.total_k / kBlock + b.b) : static_cast<int64_t>(kp.items_x) * b.h_k * b.b,
-                           DkvCfg<D>::kSmemBytes, stream);
+  return launch_persistent(diff_dq_kernel<D>, kp,
+                           varlen ? static_cast<int64_t>(b.h) * (b.total_q / kBlock + b.b) : static_cast<int64_t>(kp.items_x) * b.h * b.b,
+                           kDiffThreads, DqCfg<D>::kSmemBytes, stream);
 }
 
 }  // namespace
