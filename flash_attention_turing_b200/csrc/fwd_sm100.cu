@@ -778,29 +778,35 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           if (!(ok = mbar_wait_warp(&bars->o_full[1], no & 1, ctx))) break;
           if (!(ok = mbar_wait_warp(&bars->factors[quarter], no & 1, ctx))) break;
           tc_fence_after_sync();
-          // a row without a visible key has no factor, and its sums may hold what hidden values are
           const float other = mine[(t ^ 1) * kBlockM], inv1 = t == 0 ? inv : other, inv2 = t == 0 ? other : inv;
           const float minus = -w.lam * inv2;
           const uint32_t tO1 = tmem_base + lane_base + C::kColO + col0, tO2 = tO1 + D;
-#pragma unroll 1
+          // the accumulators of a row without a visible key may hold what hidden values are, 0 times NaN
+          const bool blind = __any_sync(0xffffffffu, inv1 == 0.f || inv2 == 0.f);
+          uint32_t a[D / 64][32], b[D / 64][32];
+#pragma unroll
           for (int q = 0; q < D / 64; ++q) {
-            uint32_t a[32], b[32];
-            tmem_ld32(tO1 + q * 32, a);
-            tmem_ld32(tO2 + q * 32, b);
-            tmem_wait_ld();
-            if (q == D / 64 - 1) {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars->o_read);
+            tmem_ld32(tO1 + q * 32, a[q]);
+            tmem_ld32(tO2 + q * 32, b[q]);
+          }
+          tmem_wait_ld();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->o_read);
+#pragma unroll
+          for (int q = 0; q < D / 64; ++q) {
+            if (blind) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) a[q][i] = inv1 == 0.f ? 0u : a[q][i], b[q][i] = inv2 == 0.f ? 0u : b[q][i];
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              a[i] = inv1 == 0.f ? 0u : __float_as_uint(fmaf(__uint_as_float(b[i]), minus, __uint_as_float(a[i]) * inv1));
-            store(orow, p.o_row_stride, a, col0 + q * 32);
+              a[q][i] = __float_as_uint(fmaf(__uint_as_float(b[q][i]), minus, __uint_as_float(a[q][i]) * inv1));
+            store(orow, p.o_row_stride, a[q], col0 + q * 32);
             if (o2row != nullptr) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) b[i] = inv2 == 0.f ? 0u : __float_as_uint(__uint_as_float(b[i]) * inv2);
-              store(o2row, p.o2_row_stride, b, col0 + q * 32);
+              for (int i = 0; i < 32; ++i) b[q][i] = __float_as_uint(__uint_as_float(b[q][i]) * inv2);
+              store(o2row, p.o2_row_stride, b[q], col0 + q * 32);
             }
           }
           ++no;

@@ -27,37 +27,35 @@ import torch
 from . import _ext
 
 
-def _tensor(x, name: str) -> None:
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-
-
-def _tables(block_table, cache_seqlens, page_refs) -> None:
-    for x, name in ((block_table, "block_table"), (cache_seqlens, "cache_seqlens"), (page_refs, "page_refs")):
-        _tensor(x, name)
-
-
-def _caches(caches) -> list:
+def _call(name: str, caches, tensors: dict, *args):
+    """The binding's function; where it does not take the types it is given, the argument to blame."""
     if isinstance(caches, torch.Tensor):
         raise TypeError("caches must be a sequence of tensors: k and v of every layer")
-    caches = list(caches)
-    for x in caches:
-        _tensor(x, "every cache")
-    return caches
+    lists = () if caches is None else (caches if type(caches) is list else list(caches),)
+    try:
+        return getattr(_ext.load(), name)(*lists, *tensors.values(), *args)
+    except TypeError:
+        for x in lists[0] if lists else ():
+            if not isinstance(x, torch.Tensor):
+                raise TypeError("every cache must be a torch.Tensor") from None
+        for key, x in tensors.items():
+            if not isinstance(x, torch.Tensor):
+                raise TypeError(f"{key} must be a torch.Tensor") from None
+        raise
 
 
 def kvcache_reserve(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor,
                     new_tokens: Union[int, torch.Tensor], page_size: int) -> torch.Tensor:
     """Gives every row the pages that ``cache_seqlens + new_tokens`` tokens need (an int for all rows, or int32 (batch,); negative
-    entries count as 0).  Returns bool (batch,): whether the row has them.  Rows are served in order while the free pages last, each
+    entries count as 0; 0 for rows that are not in use).  Returns bool (batch,): whether the row has them.  Rows are served in order while the free pages last, each
     with all it needs or nothing, and what a refused row needs is kept from the rows behind it.  A row whose columns do not suffice is
     refused and keeps nothing from others.  Calling it again for the same tokens changes nothing."""
-    _tables(block_table, cache_seqlens, page_refs)
+    tables = dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs)
     if isinstance(new_tokens, torch.Tensor):
-        return _ext.load().pages_reserve(block_table, cache_seqlens, page_refs, new_tokens, 0, page_size)
+        return _call("pages_reserve", None, tables, new_tokens, 0, page_size)
     if isinstance(new_tokens, bool) or not isinstance(new_tokens, int):
         raise TypeError("new_tokens must be an int or a torch.Tensor")
-    return _ext.load().pages_reserve(block_table, cache_seqlens, page_refs, None, new_tokens, page_size)
+    return _call("pages_reserve", None, tables, None, new_tokens, page_size)
 
 
 def kvcache_fork(caches: Sequence[torch.Tensor], block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor,
@@ -67,36 +65,25 @@ def kvcache_fork(caches: Sequence[torch.Tensor], block_table: torch.Tensor, cach
     reserved ahead are not shared.  A parent may have several children.  Returns bool (n,): whether it was done.  Not done, and
     nothing changed: a row out of range (-1 pads), a child that holds pages or that an earlier entry names, a parent that holds no page
     or fewer than its length says, or no page left for the copy (entries are served in order)."""
-    caches = _caches(caches)
-    _tables(block_table, cache_seqlens, page_refs)
-    _tensor(parents, "parents")
-    _tensor(children, "children")
-    return _ext.load().pages_fork(caches, block_table, cache_seqlens, page_refs, parents, children)
+    return _call("pages_fork", caches, dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, parents=parents,
+                                            children=children))
 
 
 def kvcache_free(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor, rows: torch.Tensor) -> None:
     """Rows ``rows`` (int32 (n,)) give their pages back and become empty.  Rows out of range (-1 pads) are skipped, empty ones
     stay as they are, and a row that is named twice is freed once."""
-    _tables(block_table, cache_seqlens, page_refs)
-    _tensor(rows, "rows")
-    _ext.load().pages_free(block_table, cache_seqlens, page_refs, rows)
+    _call("pages_free", None, dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, rows=rows))
 
 
 def kvcache_compact(caches: Sequence[torch.Tensor], block_table: torch.Tensor, page_refs: torch.Tensor) -> torch.Tensor:
     """Moves pages so that those in use are the first ones of every cache, and rewrites ``block_table`` and ``page_refs``: the i-th page
     in use that lies behind the first ``live`` pages goes to the i-th free one among them.  Returns ``live``, the number of pages in
     use, int32 (1,).  Pages that do not have to move keep their place."""
-    caches = _caches(caches)
-    _tensor(block_table, "block_table")
-    _tensor(page_refs, "page_refs")
-    return _ext.load().pages_compact(caches, block_table, page_refs)
+    return _call("pages_compact", caches, dict(block_table=block_table, page_refs=page_refs))
 
 
 def kvcache_copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """Page ``dst[i]`` of every cache becomes a copy of page ``src[i]``, int32 (n,) both.  A page may be the source of several entries.
     Returns bool (n,): whether it holds.  Not done: a page out of range (-1 pads), a destination that a later entry has too (the last one
     wins), and a source that another entry overwrites.  Neither block tables nor ``page_refs`` are looked at."""
-    caches = _caches(caches)
-    _tensor(src, "src")
-    _tensor(dst, "dst")
-    return _ext.load().pages_copy(caches, src, dst)
+    return _call("pages_copy", caches, dict(src=src, dst=dst))
