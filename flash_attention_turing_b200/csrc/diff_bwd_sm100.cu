@@ -191,22 +191,44 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
   }
 }
 
-// dlam of a head by one warp, in a fixed order: the rows' -delta_2
+// dlam of a head by one warp, in a fixed order: the rows' -delta_2, eight loads in flight.  Of one sequence where there are few, else of eight
+// sequences: many short ones would be a memory latency each (1000 texts of 24 tokens, 4 heads, D64: a training step 656 -> 486 us, the dK/dV kernel 437 -> 208).
 __device__ __forceinline__ void sum_dlam(const DiffKernelParams& p, int head, int lane) {
-  float sum = 0.f;
-  for (int batch = 0; batch < p.b; ++batch) {
-    const int rows = min(p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q, p.sq_pad);
-    const float* s = p.stats + (static_cast<int64_t>(batch) * p.h + head) * (p.sq_pad / kStatRows) * kStatFloats + 3 * kStatRows;
-    float part[8] = {};
-    for (int r0 = 0; r0 < rows; r0 += 256) {
+  constexpr int kLoads = 8;
+  auto rows_of = [&](int batch) {
+    return min(p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q, p.sq_pad);
+  };
+  auto stats_of = [&](int batch) {
+    return p.stats + (static_cast<int64_t>(batch) * p.h + head) * (p.sq_pad / kStatRows) * kStatFloats + 3 * kStatRows;
+  };
+  float part[kLoads] = {};
+  if (p.b < kLoads) {
+    for (int batch = 0; batch < p.b; ++batch) {
+      const int rows = rows_of(batch);
+      const float* s = stats_of(batch);
+      for (int r0 = 0; r0 < rows; r0 += kLoads * 32) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = r0 + i * 32 + lane;
-        if (r < rows) part[i] += s[r / kStatRows * kStatFloats + r % kStatRows];
+        for (int i = 0; i < kLoads; ++i) {
+          const int r = r0 + i * 32 + lane;
+          if (r < rows) part[i] += s[r / kStatRows * kStatFloats + r % kStatRows];
+        }
       }
     }
-    sum += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+  } else {
+    for (int first = 0; first < p.b; first += kLoads) {
+      const int mine = lane < kLoads && first + lane < p.b ? rows_of(first + lane) : 0;
+      const int most = __reduce_max_sync(0xffffffffu, mine);
+      int rows[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, i);
+      for (int r = lane; r - lane < most; r += 32) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (r < rows[i]) part[i] += stats_of(first + i)[r / kStatRows * kStatFloats + r % kStatRows];
+      }
+    }
   }
+  float sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (lane != 0) return;

@@ -40,6 +40,7 @@ DENSE = [  # b, sq, sk, h, hk, d, causal, lam
     (2, 200, 333, 6, 6, 64, True, "one"),
     (5, 384, 384, 12, 4, 64, True, "fp32"),
     (1, 1100, 1100, 16, 8, 128, True, "fp16"),
+    (11, 40, 40, 2, 1, 128, True, "one"),
 ]
 
 
@@ -151,6 +152,8 @@ VARLEN = [  # lengths q, lengths k (None: the same), h, hk, d, causal, spare row
     ([200, 77], [130, 0], 4, 4, 128, False, 5),
     ([5, 140, 1], [3, 256, 7], 2, 1, 128, True, 200),
     ([700, 33, 260], None, 8, 2, 128, True, 3),
+    ([i * 7 % 41 for i in range(21)], None, 3, 1, 64, True, 0),  # many short ones: dlam goes through them eight at a time
+    ([90] + [3] * 8, None, 2, 2, 128, False, 2),
 ]
 
 
