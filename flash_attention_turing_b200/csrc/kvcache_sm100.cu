@@ -1162,12 +1162,14 @@ struct Plan {
 // Parts of the keys in the tiled kernel of differential calls: where two or more for each row tile find an SM, of at least kLeastChunk
 // blocks and one round at full capacity.  With more row tiles a second round, the partial rows and their merge cost more than the
 // longest sequence: 4 x 500-4000 tokens, 256 new ones, H16 (128 tiles) 61 us whole and 90 in chunks of 15 blocks.  One sequence of 16384
-// tokens: 64 new ones, H8 222 -> 34 us, 512 new ones 216 -> 79; 2 x 8192, 128 new ones, H16 D64 113 -> 47.
+// tokens: 64 new ones, H8 222 -> 34 us, 512 new ones 216 -> 79; 2 x 8192, 128 new ones, H16 D64 113 -> 47.  num_splits
+// asks for fewer parts, not for more: 64 of many row tiles would be 64 times the output in scratch memory.
 constexpr int kTiledRows = 128, kTiledKeys = 128, kLeastChunk = 8;
 void plan_tiled_parts(const FaKvcacheParams* p, int* splits, int* chunk) {
   const int64_t blocks = std::max<int64_t>(1, (static_cast<int64_t>(capacity_tokens(p)) + kTiledKeys - 1) / kTiledKeys);
   const int64_t tiles = static_cast<int64_t>((p->seqlen_q + kTiledRows - 1) / kTiledRows) * (p->h / 2) * p->b;
-  const int64_t parts = std::min<int64_t>(64, p->num_splits > 0 ? p->num_splits : std::max<int64_t>(1, 148 / tiles));
+  const int64_t room = std::min<int64_t>(64, std::max<int64_t>(1, 148 / tiles));
+  const int64_t parts = p->num_splits > 0 ? std::min<int64_t>(p->num_splits, room) : room;
   int64_t each = (blocks + parts - 1) / parts;
   if (p->num_splits == 0) each = std::max<int64_t>(each, kLeastChunk);
   *splits = static_cast<int>((blocks + each - 1) / each);
