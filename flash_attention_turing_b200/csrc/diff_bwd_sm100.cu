@@ -88,7 +88,8 @@ struct DiffPreParams {
   int keys_written;     // keys per sequence that the dK/dV kernel writes
 };
 
-// As in the plain backward: an item is kPreRows rows of a head, heads fastest, d / 8 threads per item with 16-byte loads.
+// As in the plain backward: an item is kPreRows rows of a head, heads fastest, d / 8 threads per item with 16-byte loads.  Bound by memory:
+// B2 S4096 H16 D128 23 us for 102 MB read and 19 written, which stay in L2 mostly.
 constexpr int kPreRows = 4;
 static_assert(kClearThreads == 256, "the clearing threads are those of the preprocess kernel");
 __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
@@ -295,6 +296,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 // its own 32 columns of S_m, so that no other thread's scores are in the way; the dQ products take their slices from there.
 // The elementwise warps go through a block map by map, dP in registers: while they are at map 2, dQ_1 of the block and S_1, dP of the
 // next one run, while they are at map 1 of the next, dQ_2 and S_2.  Nothing is double-buffered and nothing stands still.
+// B2 S4096 H16 D128 without mask 400 us by itself: 3205 clocks a block of both maps, of which the products take 1536 and the
+// special-function unit, with every fourth pair a polynomial, 1536; both are busy half of the time, instructions are issued in 0.55 of the
+// slots.  Bound by the chain barrier, TMEM load, exponentials, store of each warp; causal S8192 by the power cap (1.65 GHz).
 constexpr int kDiffThreads = 608;
 constexpr int kDiffSched = 18;
 constexpr int kDiffReaders = kComputeWarps + 2;  // elementwise warps, producer warp, issuing thread
@@ -710,6 +714,9 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
 // Per tile: scores into registers (handed back, S of the next tile is issued), exponentials, dP^T waited for (which says that the products
 // of the tile before are over, and with them their packed operands), P^T and dS_m^T written and handed over together; then dV, dK_1, dK_2
 // and dP^T of the next tile run under its exponentials.
+// B2 S4096 H16 D128 without mask 552 us by itself: 2218 clocks a tile of both maps, of which 1139 are products and 768 exponentials (tensor
+// pipe 52 % busy, shared memory 69 %, of it 53 the products' operands, issue slots 0.53).  Bound by the two legs in turn: P and dS after dP, products
+// and dP after P and dS.
 constexpr int kQRows = 64;
 constexpr int kDkvThreads = 640;
 constexpr int kLamWarp = 19;  // sums dlam of a head while the others work: at the end of a launch it would be waited for

@@ -8,7 +8,8 @@ Shapes, masks (bottom-right aligned), grouped heads, packed sequences and the KV
 ``flash_attn_varlen_func`` and ``flash_attn_with_kvcache``: fp16, head dimension 64 or 128 (maps of 32 or 64).  A model that keeps
 2 * nheads query heads of d / 2 and values of d passes ``q.view(b, s, nheads, d)``: the two maps of a head lie next to each other.
 ``lam`` holds one weight per query head, or a single one for all, fp32 or fp16, and has a gradient.  What a model puts around the
-operator (how lam is parametrised, a norm of the heads' outputs) is its own.  ``softmax_scale`` must be at least 1e-6.
+operator (how lam is parametrised, a norm of the heads' outputs) is its own.  ``softmax_scale`` must be at least 1e-6; the weights should
+lie well inside fp16's range, the type of the products that they enter.
 No counterpart in Cy-47/flash-attention-turing.
 """
 from __future__ import annotations
@@ -100,7 +101,8 @@ def flash_diff_attn_with_kvcache(
 ) -> torch.Tensor:
     """Inference step against a KV cache: appends ``k``/``v`` in place at ``cache_seqlens`` and attends ``q`` against the first
     ``cache_seqlens + seqlen_new`` tokens.  The caches (contiguous or paged), the arguments and their checks are those of
-    ``flash_attn_with_kvcache``, and a cache may be used by both.  Not differentiable."""
+    ``flash_attn_with_kvcache``, and a cache may be used by both; ``num_splits`` is honoured as there for up to 64 queries times heads of a KV
+    head and is an upper bound for more.  Not differentiable."""
     if not isinstance(lam, torch.Tensor):
         raise TypeError("lam must be a torch.Tensor")
     # An ordinary decode step: the binding makes the same checks, and returns None for whatever it does not take as it is or would
