@@ -730,7 +730,7 @@ constexpr int kMaxQStages = 8;
 struct DiffDkvBarriers {
   uint64_t kv_full, kv_free;
   uint64_t q_full[kMaxQStages], q_empty[kMaxQStages];  // Q, dO and statistics of a tile
-  uint64_t s_full, s_loaded, dp_full, ds_full, acc_full;
+  uint64_t s_full, s_loaded, dp_full[2], ds_full[2], acc_full;  // [2]: in turn, where a role may be a tile ahead
   uint64_t tail_fixed[kMaxQStages];
   uint64_t sched_full[2], sched_empty[2], sched_go;
   DiffDkvItem items[2];
@@ -803,7 +803,9 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
   float* sStats = reinterpret_cast<float*>(sOnes + C::kOnesBytes);
   DiffDkvBarriers* bars = reinterpret_cast<DiffDkvBarriers*>(sStats + C::kStages * kStatRows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kS1 = 0, kS2 = 64, kDP = 128, kP = 192, kDS1 = 224, kAccV = 256, kAccK = 256 + D;
+  constexpr int kAhead = D == 64 ? 2 : 1;  // buffers of dP^T and the packed operands
+  constexpr int kS1 = 0, kS2 = 64, kDP = 128, kP = kDP + kAhead * 64, kDS1 = kP + kAhead * 32, kAccV = kDS1 + kAhead * 32, kAccK = kAccV + D;
+  static_assert(kAccK + D <= kTmemCols, "TMEM");
 
   if (warp == kProducerWarp && lane == 0) {
     mbar_init(&bars->kv_full, 1);
@@ -815,8 +817,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
     }
     mbar_init(&bars->s_full, 1);
     mbar_init(&bars->s_loaded, kComputeWarps);
-    mbar_init(&bars->dp_full, 1);
-    mbar_init(&bars->ds_full, kComputeWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->dp_full[i], 1), mbar_init(&bars->ds_full[i], kComputeWarps);
     mbar_init(&bars->acc_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->sched_full[i], 1);
@@ -993,9 +994,10 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
         tc_commit(&bars->s_full);
       };
       auto dp = [&](int T) {  // dP^T = V dO^T - delta_1
-        product_slices<D, 128, kQRows>(tmem_base + kDP, v_addr, do_tile(T), idesc_s, 0, D / 16);
-        statistics(tmem_base + kDP, T, 2);
-        tc_commit(&bars->dp_full);
+        const uint32_t to = tmem_base + kDP + T % kAhead * 64;
+        product_slices<D, 128, kQRows>(to, v_addr, do_tile(T), idesc_s, 0, D / 16);
+        statistics(to, T, 2);
+        tc_commit(&bars->dp_full[T % kAhead]);
       };
       int T0 = 0, ni = 0;
       uint32_t tail_phase = 0;  // bit s: parity of the next tail_fixed[s] phase to wait for
@@ -1015,14 +1017,19 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
         scores(T0);
         dp(T0);
         if (w.n_it == 1) tc_commit(&bars->kv_free);
+        if (kAhead == 2 && w.n_it > 1) {
+          if (!(ok = q_full(T0 + 1))) break;
+          dp(T0 + 1);
+        }
         for (int it = 0; ok && it < w.n_it; ++it) {
           const int T = T0 + it, s = T % C::kStages;
           if (it + 1 < w.n_it) {
             if (!(ok = q_full(T + 1) && wait(&bars->s_loaded, T & 1))) break;
             tc_fence_after_sync();
             scores(T + 1);
+            if (kAhead == 2 && it + 2 == w.n_it) tc_commit(&bars->kv_free);  // K and V may be replaced
           }
-          if (!(ok = wait(&bars->ds_full, T & 1))) break;
+          if (!(ok = wait(&bars->ds_full[T % kAhead], (T / kAhead) & 1))) break;
           if (kVarlen && (w.sq % kQRows) != 0 && it % w.per_head == w.per_head - 1) {
             if (!(ok = wait(&bars->tail_fixed[s], (tail_phase >> s) & 1))) break;
             tail_phase ^= 1u << s;
@@ -1032,14 +1039,15 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
             const uint64_t bd = make_smem_desc(do_tile(T), C::kQChunkBytes, 1024);
 #pragma unroll
             for (int k = 0; k < kQRows / 16; ++k)
-              mma_ts(tmem_base + kAccV, tmem_base + kP + k * 8, desc_advance(bd, k * 2048), idesc_dv, (it == 0 && k == 0) ? 0u : 1u);
+              mma_ts(tmem_base + kAccV, tmem_base + kP + T % kAhead * 32 + k * 8, desc_advance(bd, k * 2048), idesc_dv, (it == 0 && k == 0) ? 0u : 1u);
           }
-          product_half<D, kQRows>(tmem_base + kAccK, tmem_base + kDS1, [](int k) { return k * 8; }, q_tile(T), 0, idesc_dk, it == 0);
-          product_half<D, kQRows>(tmem_base + kAccK + D / 2, tmem_base + kDP, [](int k) { return k * 16; }, q_tile(T), 1, idesc_dk, it == 0);
+          product_half<D, kQRows>(tmem_base + kAccK, tmem_base + kDS1 + T % kAhead * 32, [](int k) { return k * 8; }, q_tile(T), 0, idesc_dk, it == 0);
+          product_half<D, kQRows>(tmem_base + kAccK + D / 2, tmem_base + kDP + T % kAhead * 64, [](int k) { return k * 16; }, q_tile(T), 1, idesc_dk, it == 0);
           tc_commit(&bars->q_empty[s]);
-          if (it + 1 < w.n_it) {
-            dp(T + 1);
-            if (it + 2 == w.n_it) tc_commit(&bars->kv_free);  // K and V may be replaced
+          if (it + kAhead < w.n_it) {
+            if (kAhead == 2 && !(ok = q_full(T + 2))) break;
+            dp(T + kAhead);
+            if (kAhead == 1 && it + 2 == w.n_it) tc_commit(&bars->kv_free);  // K and V may be replaced
           }
           if (w.n_it > kGoAhead && it + kGoAhead + 1 == w.n_it) mbar_arrive(&bars->sched_go);
         }
@@ -1112,11 +1120,12 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
         };
         select(pk);
         // dP^T(T) complete: so are dV, dK of the tile before, which read the packed operands
-        if (!(ok = mbar_wait_warp(&bars->dp_full, T & 1, ctx))) break;
+        if (!(ok = mbar_wait_warp(&bars->dp_full[T % kAhead], (T / kAhead) & 1, ctx))) break;
         tc_fence_after_sync();
         uint32_t dp[16];
-        tmem_ld16(t_base + kDP + cq * 16, dp);
-        tmem_st8(t_base + kP + cq * 8, pk);
+        const uint32_t t_dp = t_base + kDP + T % kAhead * 64 + cq * 16, t_packed = t_base + T % kAhead * 32 + cq * 8;
+        tmem_ld16(t_dp, dp);
+        tmem_st8(t_packed + kP, pk);
         const float4* differences = reinterpret_cast<const float4*>(sStats + (T % C::kStages) * kStatRows + cq * 16);
         tmem_wait_ld();
         uint32_t pk2[8];
@@ -1132,9 +1141,9 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
         }
         select(pk);
         select(pk2);
-        tmem_st8(t_base + kDS1 + cq * 8, pk);
-        tmem_st8(t_base + kDP + cq * 16, pk2);
-        warp_arrive(&bars->ds_full, lane);
+        tmem_st8(t_packed + kDS1, pk);
+        tmem_st8(t_dp, pk2);
+        warp_arrive(&bars->ds_full[T % kAhead], lane);
       }
       if (!ok) break;
       // ---- epilogue: column quarters 0,1 store the halves of dV, quarters 2,3 the halves of dK * scale ----
