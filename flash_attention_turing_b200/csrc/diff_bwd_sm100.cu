@@ -252,11 +252,13 @@ __global__ void join_dlam_kernel(const float* head_dlam, int h, void* dlam, int 
 // =============================================================================================
 // products
 // =============================================================================================
-// Every fourth pair of exponentials is a polynomial on the FMA pipes (see the forward kernel)
-template <int kPairs>
-__device__ __forceinline__ void exp2_pairs(float2 (&x)[kPairs]) {
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) x[i] = i % 4 == 3 ? exp2_polynomial(x[i]) : exp2_pair(x[i]);
+// Pair i of exponentials: every kEvery-th is a polynomial on the FMA pipes (see the forward kernel).  These kernels are short of issue slots as
+// well, and a polynomial takes 13 for two: eight are best in the dQ kernel, four in the dK/dV kernel at D = 64 and eight at D = 128 (B2 S4096 H16
+// D64 causal, both at four 437 us, dQ at three, eight, none 434, 429, 436, dK/dV at eight, none 439, 444; B2 S2048 Hq16 Hkv4 D128 causal dK/dV at
+// four, eight, none 181, 176, 178).
+template <int kEvery>
+__device__ __forceinline__ float2 exp2_of_pair(int i, float2 x) {
+  return i % kEvery == kEvery - 1 ? exp2_polynomial(x) : exp2_pair(x);
 }
 
 // C = A[:, half m of d] B[:, half m of d]^T: slices of 16 columns, of tiles of kRowsA and kRowsB rows (a swizzle chunk of 64 columns is
@@ -594,7 +596,8 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
       float2 x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = ffma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, l);
-      exp2_pairs(x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = exp2_of_pair<8>(i, x[i]);
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -1062,6 +1065,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
     const int row_in_tile = quarter * 32 + lane;
     const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+    constexpr int kEvery = D == 64 ? 4 : 8;
     int T0 = 0, ni = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
@@ -1093,11 +1097,9 @@ __global__ void __launch_bounds__(kDkvThreads, 1) diff_dkdv_kernel(const __grid_
         float2 p1[8], p2[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p1[e] = fmul2(make_float2(__uint_as_float(s1[2 * e]), __uint_as_float(s1[2 * e + 1])), c2);
-          p2[e] = fmul2(make_float2(__uint_as_float(s2[2 * e]), __uint_as_float(s2[2 * e + 1])), c2);
+          p1[e] = exp2_of_pair<kEvery>(e, fmul2(make_float2(__uint_as_float(s1[2 * e]), __uint_as_float(s1[2 * e + 1])), c2));
+          p2[e] = exp2_of_pair<kEvery>(e, fmul2(make_float2(__uint_as_float(s2[2 * e]), __uint_as_float(s2[2 * e + 1])), c2));
         }
-        exp2_pairs(p1);
-        exp2_pairs(p2);
         const int cmin = max(0, min(16, cmin0 - i_rel * kQRows)), cmax = kVarlen && i_rel == per_head - 1 ? cmax_last : 16;
         const bool masked = cmin > 0 || cmax < 16;
         if (++i_rel == per_head) i_rel = 0, ++head;
