@@ -40,6 +40,8 @@ EXPORTED_SYMBOLS = (
     "fa_pages_compact",
     "fa_pages_copy",
     "fa_pages_copy_workspace_bytes",
+    "fa_pages_reserve_workspace_bytes",
+    "fa_pages_fork_workspace_bytes",
 )
 
 _i64, _i32, _f32, _vp, _sz = C.c_int64, C.c_int32, C.c_float, C.c_void_p, C.c_size_t
@@ -189,6 +191,9 @@ def lib() -> C.CDLL:
             fn.restype, fn.argtypes = C.c_int, [*args, _vp]
         l.fa_pages_copy_workspace_bytes.restype = _sz
         l.fa_pages_copy_workspace_bytes.argtypes = [caches, _i32, _i32]
+        l.fa_pages_reserve_workspace_bytes.restype = l.fa_pages_fork_workspace_bytes.restype = _sz
+        l.fa_pages_reserve_workspace_bytes.argtypes = [tables]
+        l.fa_pages_fork_workspace_bytes.argtypes = [tables, caches, _i32]
         l.fa_pages_workspace_bytes.restype = _sz
         l.fa_pages_workspace_bytes.argtypes = [_i32, _i32, _i32]
         l.fa_kvcache_num_splits.restype = C.c_int

@@ -91,10 +91,14 @@ struct ReserveParams {
   const int* new_tokens;  // (rows), or null: new_tokens_all for each
   int new_tokens_all, page_size;
   uint8_t* granted;
-  int *need, *begin, *held, *list;  // scratch: per row, per row, per row, per page
+  int *need, *begin, *held, *list;  // scratch: per row, per row, per row, per page; null: shared memory (small tables)
 };
+constexpr int kSmallRows = 1024, kSmallPages = 4096;
 
-__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const __grid_constant__ ReserveParams p) {
+__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const __grid_constant__ ReserveParams call) {
+  __shared__ int rows_scratch[3][kSmallRows], list_scratch[kSmallPages];
+  ReserveParams p = call;
+  if (p.need == nullptr) p.need = rows_scratch[0], p.begin = rows_scratch[1], p.held = rows_scratch[2], p.list = list_scratch;
   // what each row needs; a row whose columns do not suffice needs nothing and is refused
   int64_t wanted = 0;
   for (int r0 = 0; r0 < p.t.rows; r0 += kPlanThreads) {
@@ -148,6 +152,34 @@ struct ForkParams {
 };
 constexpr int kRefused = 0x7fffffff;
 
+// Whether a parent's pages can be shared, apart from what its child is; partial: the last one has to be copied
+__device__ __forceinline__ bool forkable(const FaPageTables& t, int parent, int page_size, bool& partial) {
+  const int64_t len = max(t.cache_seqlens[parent], 0), pages = pages_of(len, page_size);
+  const int held = held_pages(t, parent, pages);
+  partial = len % page_size != 0;
+  return held > 0 && held >= pages && (!partial || t.block_table[parent * t.row_stride + pages - 1] < t.num_pages);
+}
+
+// The tables of a child, by a warp; page: for the parent's last tokens, -1: its pages are full
+__device__ __forceinline__ void fork_row(const FaPageTables& t, int parent, int child, int page_size, int page) {
+  const int lane = threadIdx.x & 31;
+  const int len = max(t.cache_seqlens[parent], 0), full = len / page_size;
+  const int* from = t.block_table + parent * t.row_stride;
+  int* to = t.block_table + child * t.row_stride;
+  for (int c = lane; c < full; c += 32) {
+    const int shared = from[c];
+    to[c] = shared;
+    if (shared < t.num_pages) atomicAdd(t.page_refs + shared, 1);
+  }
+  if (lane == 0) {
+    if (page >= 0) {
+      to[full] = page;
+      t.page_refs[page] = 1;
+    }
+    t.cache_seqlens[child] = len;
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constant__ ForkParams p) {
   grid_launch_dependents();
   auto inside = [&](int row) { return row >= 0 && row < p.t.rows; };
@@ -163,12 +195,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constan
     bool valid = false, partial = false;
     if (i < p.n) {
       const int parent = p.parents[i], child = p.children[i];
-      if (inside(parent) && inside(child) && p.first[child] == i && p.t.block_table[child * p.t.row_stride] < 0) {
-        const int64_t len = max(p.t.cache_seqlens[parent], 0), pages = pages_of(len, p.page_size);
-        const int held = held_pages(p.t, parent, pages);
-        partial = len % p.page_size != 0;
-        valid = held > 0 && held >= pages && (!partial || p.t.block_table[parent * p.t.row_stride + pages - 1] < p.t.num_pages);
-      }
+      if (inside(parent) && inside(child) && p.first[child] == i && p.t.block_table[child * p.t.row_stride] < 0)
+        valid = forkable(p.t, parent, p.page_size, partial);
     }
     int total;
     const int rank = wanted + block_scan(valid && partial, total);
@@ -178,30 +206,17 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constan
   const int found = wanted > 0 ? find_free(p.t.page_refs, p.t.num_pages, wanted, p.list) : 0;
   if (threadIdx.x == 0) *p.count = found;
   __syncthreads();  // the ranks
-  const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x >> 5; i < p.n; i += kPlanWarps) {  // a warp per entry
     const int rank = p.begin[i];
     const bool granted = rank < found;  // kRefused is not, an entry that needs no page is
-    if (lane == 0) p.granted[i] = granted;
+    if ((threadIdx.x & 31) == 0) p.granted[i] = granted;
     if (!granted) continue;
-    const int parent = p.parents[i], child = p.children[i];
-    const int len = max(p.t.cache_seqlens[parent], 0), full = len / p.page_size;
-    const int* from = p.t.block_table + parent * p.t.row_stride;
-    int* to = p.t.block_table + child * p.t.row_stride;
-    for (int c = lane; c < full; c += 32) {
-      const int page = from[c];
-      to[c] = page;
-      if (page < p.t.num_pages) atomicAdd(p.t.page_refs + page, 1);
+    const int parent = p.parents[i], page = rank >= 0 ? p.list[rank] : -1;
+    if ((threadIdx.x & 31) == 0 && rank >= 0) {
+      const int len = max(p.t.cache_seqlens[parent], 0), full = len / p.page_size;
+      p.moves[rank] = PageMove{p.t.block_table[parent * p.t.row_stride + full], page, (len - full * p.page_size) * p.token_bytes};
     }
-    if (lane == 0) {
-      if (rank >= 0) {
-        const int page = p.list[rank];
-        to[full] = page;
-        p.t.page_refs[page] = 1;
-        p.moves[rank] = PageMove{from[full], page, (len - full * p.page_size) * p.token_bytes};
-      }
-      p.t.cache_seqlens[child] = len;
-    }
+    fork_row(p.t, parent, p.children[i], p.page_size, page);
   }
 }
 
@@ -394,6 +409,112 @@ __global__ void __launch_bounds__(kCopyThreads) copy_few_kernel(const __grid_con
                       static_cast<int64_t>(chunk) * kChunk + threadIdx.x * 16, p.page_bytes);
 }
 
+// Few forks (kFewForks at most): each CTA makes the plan for itself and copies chunks of one entry in one cache; the
+// last CTA that has made it writes the tables, which nobody reads any more.  One launch and no scratch memory: 8 forks in 4 caches
+// take the host 6.0 us where the two kernels took 10.5.  Of 48 entries in
+// 16 caches 1536 CTAs would make the plan, 25 us where the two kernels take 11.
+constexpr int kFewForks = 32, kFewForkCtas = 4 * 148;
+struct FewForkParams {
+  uint8_t* base[kMaxCaches];
+  int64_t page_stride[kMaxCaches];
+  FaPageTables t;
+  const int *parents, *children;
+  uint8_t* granted;
+  int64_t token_bytes;
+  int* counter;  // zero before and after
+  int caches, chunks, ctas, n, page_size;  // ctas: for the chunks of a page of a cache
+};
+template <int kUnroll>
+__global__ void __launch_bounds__(kCopyThreads) fork_few_kernel(const __grid_constant__ FewForkParams p) {
+  constexpr int kChunk = kUnroll * kCopyThreads * 16, kWarps = kCopyThreads / 32;
+  __shared__ int parents[kFewForks], children[kFewForks], pages[kFewForks], warp_sums[kWarps];
+  __shared__ uint64_t valid_mask, partial_mask;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) valid_mask = partial_mask = 0;
+  if (tid < p.n) parents[tid] = p.parents[tid], children[tid] = p.children[tid];
+  __syncthreads();
+  if (tid < p.n) {
+    const int parent = parents[tid], child = children[tid];
+    auto inside = [&](int row) { return row >= 0 && row < p.t.rows; };
+    bool valid = inside(parent) && inside(child), partial = false;
+    for (int i = 0; i < tid; ++i) valid &= !(children[i] == child && inside(parents[i]));
+    if (valid && p.t.block_table[child * p.t.row_stride] < 0 && forkable(p.t, parent, p.page_size, partial)) {
+      atomicOr(reinterpret_cast<unsigned long long*>(&valid_mask), 1ull << tid);
+      if (partial) atomicOr(reinterpret_cast<unsigned long long*>(&partial_mask), 1ull << tid);
+    }
+  }
+  __syncthreads();
+  const uint64_t valid = valid_mask, copies = valid_mask & partial_mask;
+  const int want = __popcll(copies);
+  // the first `want` free pages, as find_free()
+  int found = 0;
+  for (int base = 0; base < p.t.num_pages && found < want; base += kCopyThreads * kPagesPerThread) {
+    const int first = base + tid * kPagesPerThread;
+    bool is_free[kPagesPerThread];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPagesPerThread; ++i) {
+      is_free[i] = first + i < p.t.num_pages && p.t.page_refs[first + i] <= 0;
+      mine += is_free[i];
+    }
+    int sum = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += other;
+    }
+    __syncthreads();  // the sums of the round before have been read
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    int at = found + sum - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = warp_sums[i];
+      if (i < warp) at += w;
+      total += w;
+    }
+#pragma unroll
+    for (int i = 0; i < kPagesPerThread; ++i) {
+      if (is_free[i] && at < want) pages[at] = first + i;
+      at += is_free[i];
+    }
+    found += total;
+  }
+  found = min(found, want);
+  // whether entry i is done, and the page of its copy (-1: it needs none)
+  auto plan = [&](int i, int& page) {
+    const int rank = __popcll(copies & ((1ull << i) - 1));
+    const bool needs = (copies >> i & 1) != 0;
+    page = needs && rank < found ? pages[rank] : -1;
+    return (valid >> i & 1) != 0 && (!needs || rank < found);
+  };
+  const int per_entry = p.caches * p.ctas;
+  const int entry = blockIdx.x / per_entry, rest = blockIdx.x - entry * per_entry, cache = rest / p.ctas;
+  int src = 0, dst = -1, len = 0;
+  __syncthreads();  // the pages
+  if (plan(entry, dst) && dst >= 0) {
+    len = max(p.t.cache_seqlens[parents[entry]], 0);
+    src = p.t.block_table[parents[entry] * p.t.row_stride + len / p.page_size];
+  }
+  __threadfence();
+  __syncthreads();  // all that this CTA reads of the tables has been read
+  const bool last = __syncthreads_or(tid == 0 && atomicAdd(p.counter, 1) == static_cast<int>(gridDim.x) - 1);
+  const int64_t bytes = len % p.page_size * p.token_bytes;
+  if (dst >= 0) {
+    for (int64_t at = static_cast<int64_t>(rest - cache * p.ctas) * kChunk; at < bytes; at += static_cast<int64_t>(p.ctas) * kChunk)
+      copy_chunk<kUnroll>(p.base[cache] + src * p.page_stride[cache], p.base[cache] + dst * p.page_stride[cache], at + tid * 16, bytes);
+  }
+  if (!last) return;
+  __threadfence();
+  if (tid == 0) *p.counter = 0;
+  for (int i = warp; i < p.n; i += kWarps) {
+    int page;
+    const bool done = plan(i, page);
+    if (lane == 0) p.granted[i] = done;
+    if (done) fork_row(p.t, parents[i], children[i], p.page_size, page);
+  }
+}
+
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Carves the workspace up; with base == nullptr only the size is wanted
@@ -478,6 +599,36 @@ int launch_moves(const FaPageCaches* c, const PageMove* moves, const int* count,
   return FA_OK;
 }
 
+// CTAs for each cache of an entry: all of them are resident together, and they read 32 MB of counts between them at most
+int few_fork_ctas(const FaPageCaches* c, int n, int* units, int* chunks) {
+  *units = chunk_units(n * c->count * c->page_bytes, 148);
+  const int64_t chunk = *units * kCopyThreads * 16;
+  *chunks = static_cast<int>((c->page_bytes + chunk - 1) / chunk);
+  return std::min(*chunks, kFewForkCtas / (n * c->count));
+}
+bool forks_few(const FaPageTables* t, const FaPageCaches* c, int n) {
+  if (n < 1 || n > kFewForks || c->count < 1 || c->count > kMaxCaches || c->page_bytes < 16 || c->page_bytes >= (1 << 30)) return false;
+  int units, chunks;
+  const int64_t ctas = few_fork_ctas(c, n, &units, &chunks);
+  return ctas >= 1 && n * c->count * ctas * t->num_pages <= (8 << 20);
+}
+
+int launch_few_forks(const FaPageTables* t, const FaPageCaches* c, const int* parents, const int* children, int n, int page_size,
+                     uint8_t* granted, cudaStream_t stream) {
+  FewForkParams p = {};
+  for (int i = 0; i < c->count; ++i) p.base[i] = static_cast<uint8_t*>(c->base[i]), p.page_stride[i] = c->page_stride[i];
+  p.t = *t, p.parents = parents, p.children = children, p.granted = granted, p.caches = c->count, p.n = n, p.page_size = page_size;
+  p.token_bytes = c->page_bytes / page_size;
+  p.counter = next_sched_slot(stream);
+  if (p.counter == nullptr) return set_error(FA_ERR_CUDA, "fa_pages_fork: device attributes not available");
+  int units;
+  p.ctas = few_fork_ctas(c, n, &units, &p.chunks);
+  const auto kernel = units == 8 ? fork_few_kernel<8> : units == 2 ? fork_few_kernel<2> : fork_few_kernel<1>;
+  kernel<<<n * c->count * p.ctas, kCopyThreads, 0, stream>>>(p);
+  FA_CHECK_CUDA(cudaGetLastError());
+  return FA_OK;
+}
+
 bool copies_few(const FaPageCaches* c, int n) {  // the items are counted in 32 bits
   return n <= kFewPages && c->count <= kMaxCaches && static_cast<int64_t>(n) * c->count * (c->page_bytes / 4096 + 1) < (1 << 30);
 }
@@ -504,19 +655,32 @@ extern "C" size_t fa_pages_copy_workspace_bytes(const FaPageCaches* caches, int3
   return fa::workspace_bytes(0, num_pages, n);
 }
 
+extern "C" size_t fa_pages_reserve_workspace_bytes(const FaPageTables* t) {
+  if (t == nullptr || t->rows < 0 || t->num_pages < 0 || (t->rows <= fa::kSmallRows && t->num_pages <= fa::kSmallPages)) return 0;
+  return fa::workspace_bytes(t->rows, t->num_pages, 0);
+}
+
+extern "C" size_t fa_pages_fork_workspace_bytes(const FaPageTables* t, const FaPageCaches* caches, int32_t n) {
+  if (t == nullptr || caches == nullptr || t->rows < 0 || t->num_pages < 0 || n < 0 || fa::forks_few(t, caches, n)) return 0;
+  return fa::workspace_bytes(t->rows, t->num_pages, n);
+}
+
 extern "C" int fa_pages_reserve(const FaPageTables* t, const int32_t* new_tokens, int32_t new_tokens_all, int32_t page_size, uint8_t* granted,
                                 void* workspace, size_t bytes, fa_stream_t stream) {
   using namespace fa;
   int rc = check_tables(t, true, "fa_pages_reserve");
   if (rc != FA_OK) return rc;
   FA_CHECK_ARG(page_size >= 1 && granted != nullptr, "fa_pages_reserve: bad page_size or granted");
-  rc = check_workspace(workspace, bytes, workspace_bytes(t->rows, t->num_pages, 0), "fa_pages_reserve");
+  const bool needs = fa_pages_reserve_workspace_bytes(t) > 0;
+  if (needs || workspace != nullptr) rc = check_workspace(workspace, bytes, workspace_bytes(t->rows, t->num_pages, 0), "fa_pages_reserve");
   if (rc != FA_OK) return rc;
   rc = check_device_sm100();
   if (rc != FA_OK) return rc;
-  Carver c{static_cast<uint8_t*>(workspace)};
   ReserveParams p{*t, new_tokens, new_tokens_all, page_size, granted};
-  p.need = c.take<int>(t->rows), p.begin = c.take<int>(t->rows), p.held = c.take<int>(t->rows), p.list = c.take<int>(t->num_pages);
+  if (needs) {
+    Carver c{static_cast<uint8_t*>(workspace)};
+    p.need = c.take<int>(t->rows), p.begin = c.take<int>(t->rows), p.held = c.take<int>(t->rows), p.list = c.take<int>(t->num_pages);
+  }
   reserve_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   FA_CHECK_CUDA(cudaGetLastError());
   return FA_OK;
@@ -533,9 +697,11 @@ extern "C" int fa_pages_fork(const FaPageTables* t, const FaPageCaches* caches, 
                "fa_pages_fork: the bytes of a token must be a multiple of 16");
   if (n == 0) return FA_OK;
   FA_CHECK_ARG(parents && children && granted, "fa_pages_fork: parents, children, granted must be non-NULL");
-  rc = check_workspace(workspace, bytes, workspace_bytes(t->rows, t->num_pages, n), "fa_pages_fork");
+  const bool few = forks_few(t, caches, n);
+  if (!few || workspace != nullptr) rc = check_workspace(workspace, bytes, workspace_bytes(t->rows, t->num_pages, n), "fa_pages_fork");
   if (rc == FA_OK) rc = check_device_sm100();
   if (rc != FA_OK) return rc;
+  if (few) return launch_few_forks(t, caches, parents, children, n, page_size, granted, stream);
   Carver c{static_cast<uint8_t*>(workspace)};
   ForkParams p{*t, parents, children, n, page_size, caches->page_bytes / page_size, granted};
   p.first = c.take<int>(t->rows), p.begin = c.take<int>(n), p.list = c.take<int>(t->num_pages);

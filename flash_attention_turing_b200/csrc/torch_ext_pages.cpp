@@ -59,12 +59,14 @@ struct Caches {
       TORCH_CHECK(t.device() == device && t.dim() == first.dim() && t.size(0) == pages && t.size(1) == page_size &&
                       t.numel() == first.numel() && t.element_size() == first.element_size(),
                   "caches must have the same device, shape and element size");
-      int64_t stride = 1;
-      for (int64_t i = t.dim() - 1; i >= 1; --i) {
-        TORCH_CHECK(t.size(i) == 1 || t.stride(i) == stride, "a page must be contiguous in every cache");
-        stride *= t.size(i);
+      if (!t.is_contiguous()) {
+        int64_t stride = 1;
+        for (int64_t i = t.dim() - 1; i >= 1; --i) {
+          TORCH_CHECK(t.size(i) == 1 || t.stride(i) == stride, "a page must be contiguous in every cache");
+          stride *= t.size(i);
+        }
+        TORCH_CHECK(pages <= 1 || t.stride(0) >= elements, "pages of a cache must not overlap");
       }
-      TORCH_CHECK(pages <= 1 || t.stride(0) >= elements, "pages of a cache must not overlap");
       const int64_t bytes = pages <= 1 ? c.page_bytes : t.stride(0) * t.element_size();
       TORCH_CHECK(bytes % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "pages must be aligned to 16 bytes");
       base.push_back(t.data_ptr());
@@ -74,6 +76,15 @@ struct Caches {
     c.count = static_cast<int32_t>(base.size());
   }
   bool empty() const { return pages == 0 || c.page_bytes == 0; }
+};
+
+struct Scratch {  // none where no bytes are wanted
+  at::Tensor memory;
+  void* data = nullptr;
+  size_t bytes;
+  Scratch(size_t wanted, const at::Tensor& like) : bytes(wanted) {
+    if (wanted > 0) memory = scratch(wanted, like), data = memory.data_ptr();
+  }
 };
 
 at::Tensor flags(int64_t n, const at::Tensor& like) { return torch::empty({n}, like.options().dtype(at::kBool)); }
@@ -94,9 +105,9 @@ at::Tensor pages_reserve(at::Tensor block_table, at::Tensor cache_seqlens, at::T
   at::Tensor granted = flags(t.rows, block_table);
   if (t.rows == 0) return granted;
   TORCH_CHECK(t.columns >= 1 && t.num_pages >= 1, "block_table and page_refs must not be empty");
-  at::Tensor ws = scratch(fa_pages_workspace_bytes(t.rows, t.num_pages, 0), block_table);
+  const Scratch ws(fa_pages_reserve_workspace_bytes(&t), block_table);
   check_rc(fa_pages_reserve(&t, tokens, static_cast<int32_t>(new_tokens_all), static_cast<int32_t>(page_size), flag_ptr(granted),
-                            ws.data_ptr(), ws.numel(), current_stream()),
+                            ws.data, ws.bytes, current_stream()),
            "fa_pages_reserve");
   return granted;
 }
@@ -119,9 +130,9 @@ at::Tensor pages_fork(std::vector<at::Tensor> caches, at::Tensor block_table, at
   if (parents.numel() == 0) return granted;
   if (t.rows == 0 || t.columns == 0 || c.empty()) return granted.zero_();
   const int32_t n = static_cast<int32_t>(parents.numel());
-  at::Tensor ws = scratch(fa_pages_workspace_bytes(t.rows, t.num_pages, n), block_table);
+  const Scratch ws(fa_pages_fork_workspace_bytes(&t, &c.c, n), block_table);
   check_rc(fa_pages_fork(&t, &c.c, parents.data_ptr<int>(), children.data_ptr<int>(), n, static_cast<int32_t>(c.page_size),
-                         flag_ptr(granted), ws.data_ptr(), ws.numel(), current_stream()),
+                         flag_ptr(granted), ws.data, ws.bytes, current_stream()),
            "fa_pages_fork");
   return granted;
 }
@@ -141,8 +152,8 @@ at::Tensor pages_compact(std::vector<at::Tensor> caches, at::Tensor block_table,
   c10::cuda::CUDAGuard guard(c.device);
   at::Tensor live = torch::empty({1}, page_refs.options());
   if (t.rows == 0 || t.columns == 0 || c.empty()) return live.zero_();
-  at::Tensor ws = scratch(fa_pages_workspace_bytes(t.rows, t.num_pages, 0), block_table);
-  check_rc(fa_pages_compact(&t, &c.c, live.data_ptr<int>(), ws.data_ptr(), ws.numel(), current_stream()), "fa_pages_compact");
+  const Scratch ws(fa_pages_workspace_bytes(t.rows, t.num_pages, 0), block_table);
+  check_rc(fa_pages_compact(&t, &c.c, live.data_ptr<int>(), ws.data, ws.bytes, current_stream()), "fa_pages_compact");
   return live;
 }
 
@@ -156,10 +167,9 @@ at::Tensor pages_copy(std::vector<at::Tensor> caches, at::Tensor src, at::Tensor
   if (src.numel() == 0) return done;
   if (c.empty()) return done.zero_();
   const int32_t n = static_cast<int32_t>(src.numel());
-  const size_t bytes = fa_pages_copy_workspace_bytes(&c.c, static_cast<int32_t>(c.pages), n);
-  at::Tensor ws = bytes > 0 ? scratch(bytes, src) : at::Tensor();
+  const Scratch ws(fa_pages_copy_workspace_bytes(&c.c, static_cast<int32_t>(c.pages), n), src);
   check_rc(fa_pages_copy(&c.c, static_cast<int32_t>(c.pages), src.data_ptr<int>(), dst.data_ptr<int>(), n, flag_ptr(done),
-                         bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+                         ws.data, ws.bytes, current_stream()),
            "fa_pages_copy");
   return done;
 }

@@ -27,21 +27,20 @@ import torch
 from . import _ext
 
 
-def _call(name: str, caches, tensors: dict, *args):
-    """The binding's function; where it does not take the types it is given, the argument to blame."""
+def _caches(caches) -> list:
     if isinstance(caches, torch.Tensor):
         raise TypeError("caches must be a sequence of tensors: k and v of every layer")
-    lists = () if caches is None else (caches if type(caches) is list else list(caches),)
-    try:
-        return getattr(_ext.load(), name)(*lists, *tensors.values(), *args)
-    except TypeError:
-        for x in lists[0] if lists else ():
-            if not isinstance(x, torch.Tensor):
-                raise TypeError("every cache must be a torch.Tensor") from None
-        for key, x in tensors.items():
-            if not isinstance(x, torch.Tensor):
-                raise TypeError(f"{key} must be a torch.Tensor") from None
-        raise
+    return caches if type(caches) is list else list(caches)
+
+
+def _blame(caches, **tensors) -> None:
+    """The binding did not take the types that it was given: names the argument that is not a tensor, if there is one."""
+    for x in caches:
+        if not isinstance(x, torch.Tensor):
+            raise TypeError("every cache must be a torch.Tensor") from None
+    for key, x in tensors.items():
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{key} must be a torch.Tensor") from None
 
 
 def kvcache_reserve(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor,
@@ -50,12 +49,15 @@ def kvcache_reserve(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page
     entries count as 0; 0 for rows that are not in use).  Returns bool (batch,): whether the row has them.  Rows are served in order while the free pages last, each
     with all it needs or nothing, and what a refused row needs is kept from the rows behind it.  A row whose columns do not suffice is
     refused and keeps nothing from others.  Calling it again for the same tokens changes nothing."""
-    tables = dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs)
-    if isinstance(new_tokens, torch.Tensor):
-        return _call("pages_reserve", None, tables, new_tokens, 0, page_size)
-    if isinstance(new_tokens, bool) or not isinstance(new_tokens, int):
+    each = isinstance(new_tokens, torch.Tensor)
+    if not each and (isinstance(new_tokens, bool) or not isinstance(new_tokens, int)):
         raise TypeError("new_tokens must be an int or a torch.Tensor")
-    return _call("pages_reserve", None, tables, None, new_tokens, page_size)
+    try:
+        return _ext.load().pages_reserve(block_table, cache_seqlens, page_refs, new_tokens if each else None, 0 if each else new_tokens,
+                                         page_size)
+    except TypeError:
+        _blame((), block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs)
+        raise
 
 
 def kvcache_fork(caches: Sequence[torch.Tensor], block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor,
@@ -65,25 +67,43 @@ def kvcache_fork(caches: Sequence[torch.Tensor], block_table: torch.Tensor, cach
     reserved ahead are not shared.  A parent may have several children.  Returns bool (n,): whether it was done.  Not done, and
     nothing changed: a row out of range (-1 pads), a child that holds pages or that an earlier entry names, a parent that holds no page
     or fewer than its length says, or no page left for the copy (entries are served in order)."""
-    return _call("pages_fork", caches, dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, parents=parents,
-                                            children=children))
+    caches = _caches(caches)
+    try:
+        return _ext.load().pages_fork(caches, block_table, cache_seqlens, page_refs, parents, children)
+    except TypeError:
+        _blame(caches, block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, parents=parents, children=children)
+        raise
 
 
 def kvcache_free(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor, rows: torch.Tensor) -> None:
     """Rows ``rows`` (int32 (n,)) give their pages back and become empty.  Rows out of range (-1 pads) are skipped, empty ones
     stay as they are, and a row that is named twice is freed once."""
-    _call("pages_free", None, dict(block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, rows=rows))
+    try:
+        _ext.load().pages_free(block_table, cache_seqlens, page_refs, rows)
+    except TypeError:
+        _blame((), block_table=block_table, cache_seqlens=cache_seqlens, page_refs=page_refs, rows=rows)
+        raise
 
 
 def kvcache_compact(caches: Sequence[torch.Tensor], block_table: torch.Tensor, page_refs: torch.Tensor) -> torch.Tensor:
     """Moves pages so that those in use are the first ones of every cache, and rewrites ``block_table`` and ``page_refs``: the i-th page
     in use that lies behind the first ``live`` pages goes to the i-th free one among them.  Returns ``live``, the number of pages in
     use, int32 (1,).  Pages that do not have to move keep their place."""
-    return _call("pages_compact", caches, dict(block_table=block_table, page_refs=page_refs))
+    caches = _caches(caches)
+    try:
+        return _ext.load().pages_compact(caches, block_table, page_refs)
+    except TypeError:
+        _blame(caches, block_table=block_table, page_refs=page_refs)
+        raise
 
 
 def kvcache_copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """Page ``dst[i]`` of every cache becomes a copy of page ``src[i]``, int32 (n,) both.  A page may be the source of several entries.
     Returns bool (n,): whether it holds.  Not done: a page out of range (-1 pads), a destination that a later entry has too (the last one
     wins), and a source that another entry overwrites.  Neither block tables nor ``page_refs`` are looked at."""
-    return _call("pages_copy", caches, dict(src=src, dst=dst))
+    caches = _caches(caches)
+    try:
+        return _ext.load().pages_copy(caches, src, dst)
+    except TypeError:
+        _blame(caches, src=src, dst=dst)
+        raise

@@ -405,7 +405,8 @@ int fa_diff_kvcache(const FaDiffKvcacheParams* p, int32_t* verdict, int32_t toke
 /* and -1 behind them; page_refs[p]: how many rows hold page p, 0 = free.  Free pages are taken in    */
 /* ascending order.  No call synchronises; calls on the same tables have to be ordered (one stream).  */
 /* Scratch: fa_pages_workspace_bytes(rows, num_pages, entries) bytes, 256-byte aligned, not shared by   */
-/* calls that may overlap; entries: n of the call, or 0.  No counterpart in the reference.           */
+/* calls that may overlap; entries: n of the call, or 0; or NULL where the query of a call's own says 0.   */
+/* No counterpart in the reference.                                                               */
 /* ------------------------------------------------------------------------------------------- */
 typedef struct FaPageTables {
   int32_t* block_table;    /* (rows, columns), consecutive rows row_stride elements apart          */
@@ -429,6 +430,7 @@ size_t fa_pages_workspace_bytes(int32_t rows, int32_t num_pages, int32_t entries
 /* Pages for cache_seqlens[r] + new_tokens[r] tokens (new_tokens NULL: new_tokens_all each; negative counts as 0).  Rows are   */
 /* served in order while the free pages last: a row is granted all it needs, or nothing; what a refused row needs counts       */
 /* against the rows behind it.  A row whose columns do not suffice is refused and counts for nothing.  granted[r]: 1 or 0.     */
+size_t fa_pages_reserve_workspace_bytes(const FaPageTables* t);
 int fa_pages_reserve(const FaPageTables* t, const int32_t* new_tokens, int32_t new_tokens_all, int32_t page_size, uint8_t* granted,
                      void* workspace, size_t workspace_bytes, fa_stream_t stream);
 
@@ -436,6 +438,7 @@ int fa_pages_reserve(const FaPageTables* t, const int32_t* new_tokens, int32_t n
 /* tokens of a page that is not full are copied to a free page.  Entries are served in order; refused (granted[i] = 0): rows     */
 /* out of range (-1 for padding), a child that holds pages or that an earlier entry names, a parent that holds none or fewer     */
 /* than its length says, and entries for which no page is left.                                                        */
+size_t fa_pages_fork_workspace_bytes(const FaPageTables* t, const FaPageCaches* caches, int32_t n);
 int fa_pages_fork(const FaPageTables* t, const FaPageCaches* caches, const int32_t* parents, const int32_t* children, int32_t n,
                   int32_t page_size, uint8_t* granted, void* workspace, size_t workspace_bytes, fa_stream_t stream);
 

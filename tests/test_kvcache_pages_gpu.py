@@ -208,6 +208,31 @@ def test_copies_of_many_pages(n):
     c.compare()
 
 
+@pytest.mark.parametrize("n", [1, 32, 33, 300])
+def test_forks_of_many_rows(n):
+    """Up to 32 entries are looked at by every CTA, more by a kernel of their own; in either case the free pages may not suffice."""
+    rng, rows, page = random.Random(n), 350, 32
+    m = Model(rows, 4, 160, page)
+    c = Cache(m, 2, 2, 64)
+    new = [rng.choice((0, 1, 40, 64, 100)) if r < 60 else 0 for r in range(rows)]
+    got = fa.kvcache_reserve(c.table, c.lens, c.refs, _int(new), page)
+    granted = m.reserve(new)
+    assert got.tolist() == granted
+    m.lens = [x * ok for x, ok in zip(new, granted)]
+    c.lens.copy_(_int(m.lens))
+    for p in range(160):
+        m.data[p] = [(p + i) % 90 for i in range(page)]
+    c.write()
+    for _ in range(3):
+        parents = [rng.randrange(-1, 70) for _ in range(n)]
+        children = [rng.randrange(60, rows + 1) for _ in range(n)]
+        got = fa.kvcache_fork(c.caches, c.table, c.lens, c.refs, _int(parents), _int(children))
+        assert got.tolist() == m.fork(parents, children)
+        c.compare()
+        fa.kvcache_free(c.table, c.lens, c.refs, _int(children[::2]))
+        m.free(children[::2])
+
+
 def test_rows_behind_one_that_cannot_be_served():
     m = Model(5, 8, 6, 32)
     c = Cache(m)
