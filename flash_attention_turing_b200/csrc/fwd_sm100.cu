@@ -96,6 +96,7 @@ struct FwdKernelParams {
   FaDiffWeights weights;
   __half* o2;         // A_2 V, or null
   int64_t o2_batch_stride, o2_row_stride, o2_head_stride;
+  int behind_clear;   // the kernel before clears rows that this one neither reads nor writes: it is waited for at the end
   DiffSplits parts;   // splits > 1: the keys of a row tile are several items, which leave partial rows
 };
 
@@ -269,7 +270,8 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
     }
     bars->abort_flag = 0;
     fence_mbar_init();
-    grid_dependency_wait();  // a cache append, or the kernel that clears the unused rows
+    // a cache append, or the kernel that clears the unused rows
+    if (!kDiff || !p.behind_clear) grid_dependency_wait();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
@@ -878,6 +880,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
     }
     __syncthreads();
   }
+  if (kDiff && p.behind_clear && blockIdx.x == 0 && threadIdx.x == 0) grid_dependency_wait();  // this launch must not complete before it
   if (warp == kMmaWarp) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, C::kTmemCols);
@@ -1048,16 +1051,20 @@ int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool o
   kp.o2_row_stride = diff ? diff->o2_row_stride : 0;
   kp.o2_head_stride = diff ? diff->o2_head_stride : 0;
   kp.parts = parts ? *parts : DiffSplits{};
+  kp.behind_clear = 0;
   kp.status = device_status_ptr();
   if (p->flags == FA_FWD_ZERO_UNUSED_ROWS && varlen_q) {  // no other value: see the header
     const PackedRows rows{kp.o, kp.o_row_stride, kp.o_head_stride, p->total_q, p->h, p->d, p->cu_seqlens_q, p->b};
-    const int lse_heads = diff ? 2 * p->h : p->h;  // rows of A_2 V outside every sequence are read by no one
+    // differential: the backward, the only reader, looks at no LSE and no A_2 V outside the sequences.  1000 texts of 24 tokens, 16 heads D128:
+    // 578 us without the LSE of both maps, 649 with
+    const int lse_batch = diff ? 0 : p->b;
     const int sms = device_sm_count();
     if (sms <= 0) return set_error(FA_ERR_CUDA, "fa_fwd: device attributes not available");
-    const UnusedLse lse{p->lse, p->lse_row_stride, p->b, lse_heads, p->seqlen_q};
+    const UnusedLse lse{p->lse, p->lse_row_stride, lse_batch, p->h, p->seqlen_q};
     clear_unused_rows_kernel<<<sms, kClearThreads, 0, stream>>>(rows, lse, kp.status);
     FA_CHECK_CUDA(cudaGetLastError());
     overlap = true;
+    kp.behind_clear = 1;
   }
 
   if (p->d == 128) return launch_fwd<128>(kp, p->b, p->h, p->seqlen_q, p->total_q, diff != nullptr, overlap, stream);

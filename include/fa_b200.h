@@ -356,7 +356,8 @@ int fa_sum_gather(const FaSumGatherParams* p, fa_stream_t stream);
 /* with a learned weight lam_h per query head.  Shapes, masks and strides are those of the calls   */
 /* above (`base`), with these differences: q and k are cut in two along d (softmax_scale is applied */
 /* as given, (d / 2)^-1/2 is usual, at least 1e-6); base.lse holds two rows per head, (b, 2 * h, lse_row_stride),   */
-/* row 2 * head + map; a row without a visible key gets O = 0 and both LSE = 0.  No counterpart in   */
+/* row 2 * head + map; a row without a visible key gets O = 0 and both LSE = 0; FA_FWD_ZERO_UNUSED_ROWS */
+/* clears rows of O, not of the LSE.  No counterpart in                                           */
 /* the reference.                                                                                 */
 /* ------------------------------------------------------------------------------------------- */
 typedef struct FaDiffWeights {
