@@ -8,8 +8,11 @@
 // Replaces kvcache_combine_kernel / kvcache_combine_kernel_legacy of the reference
 // (csrc/flash_attn/src/kvcache_native.cu:676-780); rows whose every split is empty get O = 0 and
 // LSE = 0 as there (:727).
+#include <algorithm>
+
 #include "combine.h"
 #include "diff.cuh"
+#include "fwd.h"
 
 #define FA_WAIT_INLINE
 #include "ptx.cuh"
@@ -27,16 +30,15 @@ struct CombineArgs {
   int64_t rows, o_batch_stride, o_row_stride, o_head_stride;
   int num_splits, h, seqlen_q;
   FaDiffWeights weights;  // differential
+  const int* chunk_at;
 };
 
 // kDiff: rows (b, 2 * h + map, seqlen_q) of differential attention.  A block has its warps in pairs, for the two maps of a head; the
 // warp of map 2 leaves its row in shared memory, times -lam, and that of map 1 adds it and stores.
 template <int D, bool kDiff>
-__global__ void __launch_bounds__(kWarpsPerBlock * 32) combine_kernel(const __grid_constant__ CombineArgs a) {
+__device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t row) {
   constexpr int kPerLane = D / 32;  // 2 or 4 consecutive columns
   const int lane = threadIdx.x & 31;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5);
-  grid_dependency_wait();  // the partials
   const bool beyond = row >= a.rows;
   if (!kDiff && beyond) return;
   if constexpr (kDiff) {  // warp 2 i + map has (batch, head, position) i of the block: row (batch, 2 * head + map, position)
@@ -135,6 +137,22 @@ __global__ void __launch_bounds__(kWarpsPerBlock * 32) combine_kernel(const __gr
     *reinterpret_cast<uint32_t*>(dst) = pack_half2(acc[0], acc[1]);
   }
   if (a.lse != nullptr && lane == 0) a.lse[row] = empty ? 0.f : lse_total;
+}
+
+template <int D, bool kDiff>
+__global__ void __launch_bounds__(kWarpsPerBlock * 32) combine_kernel(const __grid_constant__ CombineArgs a) {
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5);
+  grid_dependency_wait();  // the partials
+  if constexpr (kDiff) {
+    if (a.chunk_at != nullptr && __ldcg(a.chunk_at) >= kWholeChunk) return;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock; first < a.rows; first += step, row += step) {
+      combine_row<D, true>(a, row);
+      __syncthreads();  // what the warps left in shared memory has been read
+    }
+  } else {
+    combine_row<D, false>(a, row);
+  }
 }
 
 // Merge over ranks with the partials read in place (possibly from peer GPUs): D/8 lanes per output row
@@ -300,7 +318,9 @@ namespace {
 template <bool kDiff>
 int launch(const CombineArgs& a, int d, bool overlap, cudaStream_t stream) {
   if (a.rows == 0) return FA_OK;
-  const unsigned blocks = static_cast<unsigned>((a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock);
+  // where there may be nothing to merge, four per SM: 4096 that start only to end take 7 us, these 1.5
+  const int64_t all = (a.rows + kWarpsPerBlock - 1) / kWarpsPerBlock;
+  const unsigned blocks = static_cast<unsigned>(a.chunk_at != nullptr ? std::min<int64_t>(all, 4 * 148) : all);
   const auto kernel = d == 128 ? combine_kernel<128, kDiff> : combine_kernel<64, kDiff>;
   if (overlap) {
     FA_CHECK_CUDA(launch_overlapped(kernel, dim3(blocks), kWarpsPerBlock * 32, 0, stream, a));
@@ -316,15 +336,15 @@ int launch_combine(const float* o_accum, const float* lse_accum, void* o, float*
                    int num_splits, int h, int seqlen_q, int d, int64_t o_batch_stride,
                    int64_t o_row_stride, int64_t o_head_stride, cudaStream_t stream, bool overlap) {
   return launch<false>(CombineArgs{o_accum, lse_accum, static_cast<__half*>(o), lse, rows, o_batch_stride, o_row_stride, o_head_stride,
-                                   num_splits, h, seqlen_q, {}},
+                                   num_splits, h, seqlen_q, {}, nullptr},
                        d, overlap, stream);
 }
 
 int launch_diff_combine(const float* o_accum, const float* lse_accum, void* o, float* lse, int64_t rows,
                         int num_splits, int h, int seqlen_q, int d, int64_t o_batch_stride, int64_t o_row_stride, int64_t o_head_stride,
-                        const FaDiffWeights& weights, cudaStream_t stream) {
+                        const FaDiffWeights& weights, const int* chunk_at, cudaStream_t stream) {
   return launch<true>(CombineArgs{o_accum, lse_accum, static_cast<__half*>(o), lse, rows, o_batch_stride, o_row_stride, o_head_stride,
-                                  num_splits, h, seqlen_q, weights},
+                                  num_splits, h, seqlen_q, weights, chunk_at},
                       d, true, stream);
 }
 

@@ -8,10 +8,12 @@ namespace fa {
 // Same as fa_fwd(); seqused_k_add is added to every seqused_k[b] on the device.  overlap: the previous kernel of the stream
 // lets this one start early (launch_overlapped).  checked: the host refuses lengths beyond the capacity; they are neither read nor
 // reported.  diff: differential attention, with p = &diff->base.  parts: with diff, and queries that are not packed; O and the LSE are
-// then not written.
+// then not written, unless chunk_at says so.
+constexpr int kWholeChunk = 1 << 24;
 struct DiffSplits {
   int splits = 1;
-  int chunk = 1 << 24;         // 128-key blocks of a part
+  int chunk = kWholeChunk;     // 128-key blocks of a part
+  const int* chunk_at = nullptr;  // or where the kernel before leaves them; kWholeChunk: the keys are not cut, O and the LSE are written
   int64_t rows = 0;            // b * 2 h * seqlen_q
   float* o_accum = nullptr;    // (splits, rows, d), normalised
   float* lse_accum = nullptr;  // (splits, rows), -inf: nothing there

@@ -124,7 +124,7 @@ struct __align__(16) Work {
   int k_off, bq, bk, nkb;
   int fix_v_tail;
   float lam;  // differential: the weight of the head
-  int j0, split;  // differential: the item's first key block, and its place among those of the rows
+  int j0, split;  // differential: the item's first key block, and its place among those of the rows (-1: it has all keys)
 };
 
 struct Barriers {
@@ -156,7 +156,7 @@ static_assert(sizeof(Barriers) <= 1024, "barrier block");
 static_assert((kNumThreads / 32 + 3) / 4 * 32 * 168 <= 16384, "register file of one SM sub-partition");
 
 template <int D, int kItemRows, bool kDiff>
-__device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, int head, int mpair, int split, Work& w) {
+__device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, int head, int mpair, int split, int chunk, Work& w) {
   w.mpair = mpair;
   w.batch = batch;
   w.head = head;
@@ -190,8 +190,8 @@ __device__ __forceinline__ void make_work(const FwdKernelParams& p, int batch, i
     }
     if (r0 >= w.sq) n = 0;
     if constexpr (kDiff) {
-      w.split = split, w.j0 = split * p.parts.chunk;
-      n = max(0, min(n - w.j0, p.parts.chunk));
+      w.split = split, w.j0 = max(split, 0) * chunk;
+      n = max(0, min(n - w.j0, chunk));
     }
     w.nb[t] = n;
   }
@@ -299,6 +299,11 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       // 7 % at sequence length 65536).
       bool finished = false;
       int seq = 0;  // packed sequences: the sequence of the last claimed index
+      int total = p.total_items, chunk = p.parts.chunk;
+      if constexpr (kDiff) {
+        if (p.parts.chunk_at != nullptr) chunk = __ldcg(p.parts.chunk_at);
+        if (chunk >= kWholeChunk) total /= p.parts.splits;
+      }
       for (int n = 0;; ++n) {
         const int slot = n % kSchedDepth;
         int next = blockIdx.x;  // the first item of a CTA needs no counter
@@ -308,9 +313,9 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         }
         Work it;
         it.mpair = -1;
-        while (next < p.total_items) {
-          int batch, head, mpair, split = 0;
-          if (kDiff && p.parts.splits > 1) {  // a cache: the parts of a row tile one after the other, its longest ones first
+        while (next < (kDiff ? total : p.total_items)) {
+          int batch, head, mpair, split = -1;
+          if (kDiff && chunk < kWholeChunk) {  // a cache: the parts of a row tile one after the other, its longest ones first
             const int tile = next / p.parts.splits;
             split = next - tile * p.parts.splits;
             batch = tile / (p.items_x * p.h), head = tile / p.items_x - batch * p.h, mpair = p.items_x - 1 - tile % p.items_x;
@@ -345,8 +350,8 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           }
           const int sq = p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q;
           if (mpair >= 0 && mpair * kItemRows < sq) {
-            make_work<D, kItemRows, kDiff>(p, batch, head, mpair, split, it);
-            if (p.seqused_k && p.status && head == 0 && mpair == 0 && split == 0 &&
+            make_work<D, kItemRows, kDiff>(p, batch, head, mpair, split, chunk, it);
+            if (p.seqused_k && p.status && head == 0 && mpair == 0 && split <= 0 &&
                 cache_length(p.seqused_k[batch], p.seqused_k_add, p.k_capacity, p.checked).report)
               atomicOr(p.status, kStatusCapacityClamped);
             break;
@@ -726,7 +731,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
           inv = 1.f / l;
           lse_val = (m * c + __log2f(l)) * kLn2;
         }
-        if (p.parts.splits > 1) {  // the map's rows over the item's keys, normalised, in 32 bits
+        if (w.split >= 0) {  // the map's rows over the item's keys, normalised, in 32 bits
           const int64_t part_row = (static_cast<int64_t>(w.batch) * 2 * p.h + 2 * w.head + t) * p.seqlen_q + row +
                                    w.split * p.parts.rows;
           if (row_valid) p.parts.lse_accum[part_row] = inv == 0.f ? -INFINITY : lse_val;

@@ -987,6 +987,34 @@ struct AppendParams {
   int num_arrivals;
 };
 
+// The parts of the keys of a tiled differential call, decided where the lengths are (see plan_tiled_parts)
+struct CutPlan {
+  int* chunk;           // where the answer goes, 128-key blocks or kWholeChunk; null: nobody asks
+  int tiles, splits;    // row tiles of a sequence and all heads; parts at most
+  int seqlen_new, capacity, checked;
+};
+constexpr int kTiledRows = 128, kTiledKeys = 128, kLeastChunk = 8;
+// blocks that the longest sequence has to have more than an SM's share of all: what the parts cost
+constexpr int kCutGain = 14;
+// By the threads of one block
+__device__ __forceinline__ void plan_cut(const CutPlan& p, const int* lengths, int b) {
+  __shared__ int sums[32], most[32];
+  if (p.chunk == nullptr) return;
+  int sum = 0, longest = 0;
+  for (int i = threadIdx.x; i < b; i += blockDim.x) {
+    const int n = (cache_length(lengths[i], p.seqlen_new, p.capacity, p.checked).len + kTiledKeys - 1) / kTiledKeys;
+    sum += n, longest = max(longest, n);
+  }
+  sum = __reduce_add_sync(0xffffffffu, sum), longest = __reduce_max_sync(0xffffffffu, longest);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum, most[threadIdx.x >> 5] = longest;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < static_cast<int>(blockDim.x) >> 5; ++i) sum += sums[i], longest = max(longest, most[i]);
+  const int share = static_cast<int>((static_cast<int64_t>(sum) * p.tiles + 147) / 148);
+  const int parts = min(p.splits, (longest + max(share, kLeastChunk) - 1) / max(share, kLeastChunk));
+  *p.chunk = longest > share + kCutGain ? (longest + parts - 1) / parts : kWholeChunk;
+}
+
 // By the threads of one block.
 __device__ __forceinline__ void zero_arrivals(int* arrivals, int n) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) arrivals[i] = 0;
@@ -1005,9 +1033,10 @@ __device__ __forceinline__ void tell_host(int* verdict, int token, bool fits) {
 
 // Calls without new tokens: what the append kernel does besides appending
 __global__ void __launch_bounds__(256) prepare_kernel(const int* lengths, int b, int64_t max_length, int* verdict, int token, int* arrivals,
-                                                      int num_arrivals) {
+                                                      int num_arrivals, const CutPlan cut) {
   grid_launch_dependents();
   zero_arrivals(arrivals, num_arrivals);
+  plan_cut(cut, lengths, b);
   if (verdict != nullptr) {
     const bool fits = lengths_fit(lengths, b, max_length);
     if (threadIdx.x == 0) tell_host(verdict, token, fits);
@@ -1016,7 +1045,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const int* lengths, int b,
 
 // The 16-byte units of the first step are fetched before the lengths are looked at: two memory latencies in a row instead of four
 // (lengths, the length again, the unit, the store), which is most of what a small append takes.
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p, const __grid_constant__ CutPlan cut) {
   grid_launch_dependents();
   const int unit_bits = p.d == 128 ? 4 : 3;  // d / 8 units of 16 bytes per (token, head)
   const int64_t total = (static_cast<int64_t>(p.b) * p.seqlen_new * p.h_k) << unit_bits;
@@ -1038,7 +1067,10 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     vv = *reinterpret_cast<const uint4*>(p.v_new + batch * p.vn_batch_stride + t * p.vn_row_stride + head * p.vn_head_stride + u * 8);
   };
   if (idx < total) fetch();
-  if (blockIdx.x == 0) zero_arrivals(p.arrivals, p.num_arrivals);
+  if (blockIdx.x == 0) {
+    zero_arrivals(p.arrivals, p.num_arrivals);
+    plan_cut(cut, p.cache_seqlens, p.b);
+  }
   if (p.verdict != nullptr) {  // every block looks at all lengths (b loads by its 256 threads, from L2 but for the first): no launch in between
     const bool fits = lengths_fit(p.cache_seqlens, p.b, p.max_length);
     if (blockIdx.x == 0 && threadIdx.x == 0) tell_host(p.verdict, p.token, fits);
@@ -1157,6 +1189,7 @@ struct Plan {
   int splits = 1;         // parts that the keys of a sequence are attended in (balanced kernel: at most)
   int chunk = 0;          // tiles of a split; 0: proportional ranges
   size_t lse = 0;         // scratch memory: offset of the LSE of the parts behind the parts, and the size
+  size_t chunk_at = 0;    // tiled differential calls: of the chunk that is decided on the device
   size_t bytes = 0;
 };
 // Parts of the keys in the tiled kernel of differential calls: where two or more for each row tile find an SM, of at least kLeastChunk
@@ -1164,10 +1197,24 @@ struct Plan {
 // longest sequence: 4 x 500-4000 tokens, 256 new ones, H16 (128 tiles) 61 us whole and 90 in chunks of 15 blocks.  One sequence of 16384
 // tokens: 64 new ones, H8 222 -> 34 us, 512 new ones 216 -> 79; 2 x 8192, 128 new ones, H16 D64 113 -> 47.  num_splits
 // asks for fewer parts, not for more: 64 of many row tiles would be 64 times the output in scratch memory.
-constexpr int kTiledRows = 128, kTiledKeys = 128, kLeastChunk = 8;
+// Up to kAdaptiveTiles row tiles, the kernel that appends looks at the lengths: the keys are cut, in three parts at most, where the longest
+// sequence is kCutGain blocks above an SM's share of all.  3 x 200 new on 300, 6000, 900 (H16 D64) 90 -> 54 us, 6 x 128 on 100-8000 (H16)
+// 120 -> 70; 4 x 256 on 1500-3500 (30 blocks, share 19: not cut) 64.5 -> 66.2.
+constexpr int kAdaptiveTiles = 148, kAdaptiveParts = 3;
+int64_t tiled_tiles(const FaKvcacheParams* p) {
+  return static_cast<int64_t>((p->seqlen_q + kTiledRows - 1) / kTiledRows) * (p->h / 2) * p->b;
+}
+bool cuts_adaptively(const FaKvcacheParams* p) {
+  const int64_t tiles = tiled_tiles(p);
+  return p->num_splits == 0 && p->b > 1 && tiles > 74 && tiles <= kAdaptiveTiles && capacity_tokens(p) > (kLeastChunk + kCutGain) * kTiledKeys;
+}
 void plan_tiled_parts(const FaKvcacheParams* p, int* splits, int* chunk) {
   const int64_t blocks = std::max<int64_t>(1, (static_cast<int64_t>(capacity_tokens(p)) + kTiledKeys - 1) / kTiledKeys);
-  const int64_t tiles = static_cast<int64_t>((p->seqlen_q + kTiledRows - 1) / kTiledRows) * (p->h / 2) * p->b;
+  const int64_t tiles = tiled_tiles(p);
+  if (cuts_adaptively(p)) {
+    *splits = kAdaptiveParts, *chunk = kWholeChunk;
+    return;
+  }
   const int64_t room = std::min<int64_t>(64, std::max<int64_t>(1, 148 / tiles));
   const int64_t parts = p->num_splits > 0 ? std::min<int64_t>(p->num_splits, room) : room;
   int64_t each = (blocks + parts - 1) / parts;
@@ -1183,7 +1230,8 @@ Plan plan_call(const FaKvcacheParams* p, bool diff = false) {
       if (plan.splits > 1) {
         const size_t rows = static_cast<size_t>(plan.splits) * p->b * p->h * p->seqlen_q;
         plan.lse = align_up(rows * p->d * sizeof(float), 256);
-        plan.bytes = plan.lse + align_up(rows * sizeof(float), 256);
+        plan.chunk_at = plan.lse + align_up(rows * sizeof(float), 256);
+        plan.bytes = plan.chunk_at + 256;
       }
     }
     return plan;
@@ -1305,8 +1353,13 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
   // ---- 1. append ----
   const bool appends = p->k_new && p->seqlen_new > 0;
   const int64_t max_length = (p->block_table ? static_cast<int64_t>(p->max_blocks_per_seq) : 1) * p->seqlen_cache - p->seqlen_new;
-  if (!appends && (verdict != nullptr || num_arrivals > 0)) {
-    prepare_kernel<<<1, 256, 0, stream>>>(p->cache_seqlens, p->b, max_length, verdict, token, arrivals, num_arrivals);
+  CutPlan cut = {};
+  if (diff && !uses_decode_kernel(p, diff) && cuts_adaptively(p))
+    cut = CutPlan{reinterpret_cast<int*>(scratch + plan.chunk_at), static_cast<int>(tiled_tiles(p) / p->b), plan.splits,
+                  appends ? p->seqlen_new : 0, capacity_tokens(p), verdict != nullptr};
+  const bool prepares = !appends && (verdict != nullptr || num_arrivals > 0 || cut.chunk != nullptr);
+  if (prepares) {
+    prepare_kernel<<<1, 256, 0, stream>>>(p->cache_seqlens, p->b, max_length, verdict, token, arrivals, num_arrivals, cut);
     FA_CHECK_CUDA(cudaGetLastError());
   }
   if (appends) {
@@ -1335,7 +1388,7 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
     ap.arrivals = arrivals; ap.num_arrivals = num_arrivals;
     const int64_t total = static_cast<int64_t>(p->b) * p->seqlen_new * p->h_k * (p->d / 8);
     const int blocks = static_cast<int>(std::min<int64_t>((total + 255) / 256, 148 * 8));
-    append_kernel<<<blocks, 256, 0, stream>>>(ap);
+    append_kernel<<<blocks, 256, 0, stream>>>(ap, cut);
     FA_CHECK_CUDA(cudaGetLastError());
   }
 
@@ -1366,10 +1419,11 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
     DiffSplits parts;
     parts.splits = plan.splits, parts.chunk = plan.chunk, parts.rows = static_cast<int64_t>(p->b) * p->h * p->seqlen_q;
     parts.o_accum = reinterpret_cast<float*>(scratch), parts.lse_accum = reinterpret_cast<float*>(scratch + plan.lse);
-    rc = run_fwd(&f, p->seqlen_new, stream, appends, verdict != nullptr, &tiled, &parts);
+    parts.chunk_at = cut.chunk;
+    rc = run_fwd(&f, p->seqlen_new, stream, appends || cut.chunk != nullptr, verdict != nullptr, &tiled, &parts);
     if (rc != FA_OK) return rc;
     return launch_diff_combine(parts.o_accum, parts.lse_accum, p->o, p->lse, parts.rows, plan.splits, p->h, p->seqlen_q, p->d,
-                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, stream);
+                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, cut.chunk, stream);
   }
 
   const int64_t rows_total = static_cast<int64_t>(p->b) * p->h * p->seqlen_q;
@@ -1429,7 +1483,7 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
   // ---- 3. merge ----
   if (plan.splits > 1 && diff)
     return launch_diff_combine(dp.o_accum, dp.lse_accum, p->o, p->lse, rows_total, plan.splits, p->h, p->seqlen_q, p->d,
-                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, stream);
+                               p->o_batch_stride, p->o_row_stride, p->o_head_stride, *weights, nullptr, stream);
   if (plan.splits > 1)
     return launch_combine(dp.o_accum, dp.lse_accum, p->o, p->lse, rows_total, plan.splits, p->h, p->seqlen_q, p->d,
                           p->o_batch_stride, p->o_row_stride, p->o_head_stride, stream, true);

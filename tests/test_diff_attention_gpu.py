@@ -205,6 +205,10 @@ CACHE = [  # b, new, q rows, lengths, h, hk, d, page (0: contiguous), num_splits
     (1, 70, 70, [9000], 4, 2, 128, 256, 0),       # few row tiles, a long cache: its keys in parts
     (3, 140, 140, [5, 2500, 0], 4, 1, 64, 0, 3),  # parts that some rows have no key in
     (2, 100, 100, [1000, 3000], 8, 4, 64, 256, 1),
+    (6, 130, 130, [0, 5000, 100, 7, 900, 300], 8, 2, 64, 256, 0),   # 96 row tiles, one long sequence: cut by the device's decision
+    (4, 256, 200, [4000, 10, 3000, 300], 12, 4, 128, 512, 0),
+    (6, 130, 130, [2500, 2000, 2300, 2700, 2100, 2900], 8, 2, 64, 0, 0),  # as many, nearly equal: not cut
+    (3, 0, 500, [6000, 500, 0], 8, 8, 64, 256, 0),                  # nothing to append
     (64, 1, 1, list(range(5, 645, 10)), 4, 2, 64, 256, 0),
     (40, 1, 1, list(range(100, 4100, 100)), 8, 4, 128, 256, 0),
 ]
