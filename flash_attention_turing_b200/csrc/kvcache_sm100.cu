@@ -132,7 +132,7 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c8) {
 }
 
 // What a consumer warp holds of its (up to 16) query rows: the Q fragments and the running (maximum, sum, O) over its tokens.
-template <int D, bool kDiff>
+template <int D>
 struct WarpRows {
   uint32_t qa[D / 16][4];
   int lim0, lim1;         // last visible key of fragment rows g and g + 8
@@ -141,6 +141,7 @@ struct WarpRows {
   float l0, l1;           // per-thread partial row sums
 
   // first: the row of the KV head that is row 0 here
+  template <bool kDiff>
   __device__ __forceinline__ void begin(const DecodeParams& p, int batch, int head_k, int len, int first, int rows, int lane) {
     const int g = lane >> 2;   // fragment row (and row + 8)
     const int t4 = lane & 3;   // fragment column pair
@@ -386,8 +387,8 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
     // =========================== consumers ===========================
     const int g = lane >> 2;   // fragment row (and row + 8)
     const int t4 = lane & 3;   // fragment column pair
-    WarpRows<D, kDiff> w;
-    w.begin(p, batch, head_k, len, first_row, rows, lane);
+    WarpRows<D> w;
+    w.template begin<kDiff>(p, batch, head_k, len, first_row, rows, lane);
     const float c = p.scale_log2;
     const int tok_in_tile = warp * 16;     // this warp's 16 tokens of every tile
     bool ok = true;
@@ -817,8 +818,8 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
       if (w.tile == 0 && head_k == 0 && threadIdx.x == 0 && p.status &&
           cache_length(p.cache_seqlens[w.batch], p.seqlen_new, p.capacity, p.checked).report)
         atomicOr(p.status, kStatusCapacityClamped);
-      WarpRows<D, kDiff> mine;
-      mine.begin(p, w.batch, head_k, w.len, 0, rows, lane);
+      WarpRows<D> mine;
+      mine.template begin<kDiff>(p, w.batch, head_k, w.len, 0, rows, lane);
       for (int t = 0; t < n; ++t, ++i) {
         if (!(ok = wait_full(i))) break;
         uint8_t* stage = smem + (i % C::kStages) * C::kStageBytes;
