@@ -1048,6 +1048,11 @@ __global__ void __launch_bounds__(256) prepare_kernel(const int* lengths, int b,
 // (lengths, the length again, the unit, the store), which is most of what a small append takes.
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p, const __grid_constant__ CutPlan cut) {
   grid_launch_dependents();
+  if (cut.chunk != nullptr && blockIdx.x == gridDim.x - 1) {  // a block of its own
+    plan_cut(cut, p.cache_seqlens, p.b);
+    return;
+  }
+  const unsigned blocks = gridDim.x - (cut.chunk != nullptr);
   const int unit_bits = p.d == 128 ? 4 : 3;  // d / 8 units of 16 bytes per (token, head)
   const int64_t total = (static_cast<int64_t>(p.b) * p.seqlen_new * p.h_k) << unit_bits;
   int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -1068,10 +1073,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     vv = *reinterpret_cast<const uint4*>(p.v_new + batch * p.vn_batch_stride + t * p.vn_row_stride + head * p.vn_head_stride + u * 8);
   };
   if (idx < total) fetch();
-  if (blockIdx.x == 0) {
-    zero_arrivals(p.arrivals, p.num_arrivals);
-    plan_cut(cut, p.cache_seqlens, p.b);
-  }
+  if (blockIdx.x == 0) zero_arrivals(p.arrivals, p.num_arrivals);
   if (p.verdict != nullptr) {  // every block looks at all lengths (b loads by its 256 threads, from L2 but for the first): no launch in between
     const bool fits = lengths_fit(p.cache_seqlens, p.b, p.max_length);
     if (blockIdx.x == 0 && threadIdx.x == 0) tell_host(p.verdict, p.token, fits);
@@ -1093,7 +1095,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       *reinterpret_cast<uint4*>(p.k_cache + blk * p.kc_batch_stride + row * p.kc_row_stride + head * p.kc_head_stride + u * 8) = kv;
       *reinterpret_cast<uint4*>(p.v_cache + blk * p.vc_batch_stride + row * p.vc_row_stride + head * p.vc_head_stride + u * 8) = vv;
     }
-    idx += static_cast<int64_t>(gridDim.x) * blockDim.x;
+    idx += static_cast<int64_t>(blocks) * blockDim.x;
     if (idx < total) fetch();
   }
 }
@@ -1389,7 +1391,7 @@ int run_kvcache(const FaKvcacheParams* p, const FaDiffWeights* weights, int* ver
     ap.arrivals = arrivals; ap.num_arrivals = num_arrivals;
     const int64_t total = static_cast<int64_t>(p->b) * p->seqlen_new * p->h_k * (p->d / 8);
     const int blocks = static_cast<int>(std::min<int64_t>((total + 255) / 256, 148 * 8));
-    append_kernel<<<blocks, 256, 0, stream>>>(ap, cut);
+    append_kernel<<<blocks + (cut.chunk != nullptr), 256, 0, stream>>>(ap, cut);
     FA_CHECK_CUDA(cudaGetLastError());
   }
 
