@@ -298,9 +298,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 // its own 32 columns of S_m, so that no other thread's scores are in the way; the dQ products take their slices from there.
 // The elementwise warps go through a block map by map, dP in registers: while they are at map 2, dQ_1 of the block and S_1, dP of the
 // next one run, while they are at map 1 of the next, dQ_2 and S_2.  Nothing is double-buffered and nothing stands still.
-// B2 S4096 H16 D128 without mask 400 us by itself: 3205 clocks a block of both maps, of which the products take 1536 and the
-// special-function unit, with every fourth pair a polynomial, 1536; both are busy half of the time, instructions are issued in 0.55 of the
-// slots.  Bound by the chain barrier, TMEM load, exponentials, store of each warp; causal S8192 by the power cap (1.65 GHz).
+// B2 S4096 H16 D128 without mask 400-440 us by itself: 3147 clocks a block of both maps, of which the products take 1536 and the
+// special-function unit, with every eighth pair a polynomial, 1792; the one is busy half of the time, the other 58 %, instructions are issued in
+// 0.51 of the slots.  Bound by the chain barrier, TMEM load, exponentials, store of each warp; causal S8192 by the power cap (1.65 GHz).
 constexpr int kDiffThreads = 608;
 constexpr int kDiffSched = 18;
 constexpr int kDiffReaders = kComputeWarps + 2;  // elementwise warps, producer warp, issuing thread
@@ -717,9 +717,10 @@ __global__ void __launch_bounds__(kDiffThreads, 1) diff_dq_kernel(const __grid_c
 // Per tile: scores into registers (handed back, S of the next tile is issued), exponentials, dP^T waited for (which says that the products
 // of the tile before are over, and with them their packed operands), P^T and dS_m^T written and handed over together; then dV, dK_1, dK_2
 // and dP^T of the next tile run under its exponentials.
-// B2 S4096 H16 D128 without mask 552 us by itself: 2218 clocks a tile of both maps, of which 1139 are products and 768 exponentials (tensor
-// pipe 52 % busy, shared memory 69 %, of it 53 the products' operands, issue slots 0.53).  Bound by the two legs in turn: P and dS after dP, products
-// and dP after P and dS.
+// B2 S4096 H16 D128 without mask 550-590 us by itself: 2150 clocks a tile of both maps, of which 1139 are products and 896 exponentials (tensor
+// pipe 53 % busy, shared memory 69 %, of it 53 the products' operands, issue slots 0.50).  Bound by the chain of a warp (barriers, TMEM loads, exponentials,
+// stores): with room for two of dP and the packed operands (D = 64, where the columns are 128, 256 and 320 on) the products of a tile are not waited for by
+// the next, which gained 2 %; dK_2 and dP of the next tile ahead of dV and dK_1 at D = 128 lost 3 %.
 constexpr int kQRows = 64;
 constexpr int kDkvThreads = 640;
 constexpr int kLamWarp = 19;  // sums dlam of a head while the others work: at the end of a launch it would be waited for
