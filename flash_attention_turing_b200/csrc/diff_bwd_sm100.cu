@@ -119,8 +119,10 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
   const __half* o = p.o + base(p.o_batch_stride, p.o_row_stride, p.o_head_stride);
   const __half* o2 = p.o2 + base(p.o2_batch_stride, p.o2_row_stride, p.o2_head_stride);
   const __half* dout = p.dout + base(p.do_batch_stride, p.do_row_stride, p.do_head_stride);
-  // the padding of a sequence much shorter than the longest: nothing reads statistics past its last 128-row tile
-  if (__any_sync(0xffffffffu, row0 < (sq + kBlock - 1) / kBlock * kBlock)) {
+  // Behind the last row the dK/dV kernel needs -inf up to the end of its 64-row tile, but not in packed batches, where it masks those rows; the
+  // dQ kernel does not store them.  (Up to the end of the 128-row tile: 1000 texts of 24 tokens, 16 heads D128 213 us, 111 so.)
+  const int rows = p.cu_seqlens_q ? sq : min((sq + kStatRows - 1) / kStatRows * kStatRows, p.sq_pad);
+  if (__any_sync(0xffffffffu, row0 < rows)) {
     uint4 a[kPreRows], b[kPreRows], c[kPreRows];
 #pragma unroll
     for (int i = 0; i < kPreRows; ++i) {
@@ -193,7 +195,8 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
 }
 
 // dlam of a head by one warp, in a fixed order: the rows' -delta_2, eight loads in flight.  Of one sequence where there are few, else of eight
-// sequences: many short ones would be a memory latency each (1000 texts of 24 tokens, 4 heads, D64: a training step 656 -> 486 us, the dK/dV kernel 437 -> 208).
+// sequences: many short ones would be a memory latency each (1000 texts of 24 tokens, 4 heads, D64: a training step
+// 656 -> 486 us, the dK/dV kernel 437 -> 208).
 __device__ __forceinline__ void sum_dlam(const DiffKernelParams& p, int head, int lane) {
   constexpr int kLoads = 8;
   auto rows_of = [&](int batch) {

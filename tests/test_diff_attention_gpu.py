@@ -185,6 +185,34 @@ def test_packed_sequences(lq, lk, h, hk, d, causal, spare):
     check_dlam(grads[3], (dlam, bound))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_scratch_memory_may_hold_anything(d):
+    """NaN wherever torch's allocator hands out memory: statistics of rows that do not exist are not written, and not used."""
+    gen = _gen(13)
+    lens, h, hk = [1, 65, 0, 127, 24, 200], 4, 2
+    n = sum(lens)
+    cu = torch.tensor([0] + lens).cumsum(0).int().cuda()
+    lam = _lam(gen, h)
+    packed = [_randn(gen, n, x, d) for x in (h, hk, hk, h)]
+    dense = [_randn(gen, 2, 70, x, d) for x in (h, hk, hk, h)]
+
+    def run(poison):
+        out = []
+        for x in (packed, dense):
+            leaves = [t.detach().requires_grad_() for t in (*x[:3], lam)]
+            if poison:
+                torch.cuda.empty_cache()
+                memory = torch.full((32 << 20,), 255, dtype=torch.uint8, device="cuda")
+                del memory
+            o = (fa.flash_diff_attn_varlen_func(*leaves, cu, cu, 200, 200, causal=True) if x is packed
+                 else fa.flash_diff_attn_func(*leaves, causal=True))
+            out += [o, *torch.autograd.grad(o, leaves, x[3])]
+        return out
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 CACHE = [  # b, new, q rows, lengths, h, hk, d, page (0: contiguous), num_splits
     (1, 1, 1, [0], 2, 1, 64, 0, 0),
     (3, 1, 1, [0, 63, 500], 8, 2, 128, 0, 0),
