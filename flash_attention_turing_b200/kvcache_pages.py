@@ -12,7 +12,8 @@ table, and -1 stands behind them; an unused row has length 0 and no page.  A fre
 and a step of a serving loop: ``kvcache_reserve`` for the tokens to come, the attention of every layer (which appends them),
 ``cache_seqlens += 1``, ``kvcache_fork`` and ``kvcache_free`` as sequences split and end.  The tensors are changed in place; free pages
 are taken in ascending order, so that the outcome does not depend on scheduling.  Nothing synchronises: what could not be done is told
-by a bool tensor on the device.  Calls on the same tables have to be ordered, by one stream for instance, and may be captured in a CUDA graph.
+by a bool tensor on the device.  Calls on the same tables have to be ordered, by one stream for instance, and may be captured in a CUDA
+graph (after a first call outside a capture).
 
 Pages that rows share are full, and attention only appends, so they are never written.  A row that is cut back into a shared
 page (``cache_seqlens`` lowered by hand) must not be appended to: fork it instead, which copies the page, and free the original.
