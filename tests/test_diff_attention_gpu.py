@@ -396,6 +396,32 @@ def test_decode_in_a_cuda_graph(monkeypatch):
             assert torch.equal(k_cache[i, n[i]], k[i, 0])
 
 
+def test_chunks_in_a_cuda_graph_with_other_lengths(monkeypatch):
+    """96 row tiles: whether the keys are cut is decided on the device, at every replay anew."""
+    from flash_attention_turing_b200 import flash_attention_interface as interface
+
+    monkeypatch.setattr(interface, "HOST_CAPACITY_CHECK", False)
+    gen = _gen(14)
+    b, rows, h, hk, d, capacity = 6, 130, 8, 2, 64, 5376
+    k_cache, v_cache, lam = _randn(gen, b, capacity, hk, d), _randn(gen, b, capacity, hk, d), _lam(gen, h)
+    q, k, v = _randn(gen, b, rows, h, d), _randn(gen, b, rows, hk, d), _randn(gen, b, rows, hk, d)
+    lens = torch.zeros(b, dtype=torch.int32, device="cuda")
+
+    def step():
+        return fa.flash_diff_attn_with_kvcache(q, k_cache, v_cache, lam, k, v, cache_seqlens=lens, causal=True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for lengths in ([0] * 6, [5200, 10, 0, 700, 300, 90], [2000, 2100, 1900, 2050, 1800, 2200], [3, 4000, 8, 100, 5246, 60]):
+        lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        for i, n in enumerate(lengths):
+            check(out[i], sequence(q[i], k_cache[i, :n + rows], v_cache[i, :n + rows], lam, True)["out"], f"{lengths} {i}")
+
+
 def test_parameter_and_the_class_behind_the_native_node():
     gen = _gen(14)
     q, k, v, lam = _randn(gen, 1, 40, 2, 64), _randn(gen, 1, 40, 2, 64), _randn(gen, 1, 40, 2, 64), _lam(gen, 2)
