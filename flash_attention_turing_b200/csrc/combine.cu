@@ -50,9 +50,9 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t row) {
   const float* lse_row = a.lse_accum + row;
   const float first = lane < a.num_splits ? lse_row[lane * a.rows] : -INFINITY;
   float mx = first;
-  for (int s = lane + 32; s < a.num_splits; s += 32) mx = fmaxf(mx, lse_row[s * a.rows]);
+  for (int s = lane + 32; s < a.num_splits; s += 32) mx = fmax_nan(mx, lse_row[s * a.rows]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  for (int off = 16; off > 0; off >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   float sum = 0.f;
   if (mx != -INFINITY) {
     if (lane < a.num_splits) sum += __expf(first - mx);

@@ -261,7 +261,7 @@ __global__ void join_dlam_kernel(const float* head_dlam, int h, void* dlam, int 
 // four, eight, none 181, 176, 178).
 template <int kEvery>
 __device__ __forceinline__ float2 exp2_of_pair(int i, float2 x) {
-  return i % kEvery == kEvery - 1 ? exp2_polynomial(x) : exp2_pair(x);
+  return i % kEvery == kEvery - 1 ? exp2_polynomial<true>(x) : exp2_pair(x);
 }
 
 // C = A[:, half m of d] B[:, half m of d]^T: slices of 16 columns, of tiles of kRowsA and kRowsB rows (a swizzle chunk of 64 columns is

@@ -623,14 +623,16 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
         // four independent chains: a single running maximum would be bound by the latency of 64 dependent ops
         auto max32 = [&](const uint32_t (&v)[32], float a) {
           float a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+          // differential: a NaN score is the maximum, see exp2_polynomial()
+          auto max3 = [](float x, float y, float z) { return kDiff ? fmax3_nan(x, y, z) : fmax3(x, y, z); };
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
-            a = fmax3(a, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            a1 = fmax3(a1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-            a2 = fmax3(a2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
-            a3 = fmax3(a3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+            a = max3(a, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            a1 = max3(a1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            a2 = max3(a2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
+            a3 = max3(a3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
           }
-          return fmaxf(fmax3(a, a1, a2), a3);
+          return kDiff ? fmax_nan(max3(a, a1, a2), a3) : fmaxf(max3(a, a1, a2), a3);
         };
 
         // ---- pass 1: row maximum over all 128 columns, one round of loads ----
@@ -660,9 +662,10 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
 
         // lazy reference maximum, branch-free
         const bool fresh = (m == -INFINITY);
-        const bool need = !fresh && (mx - m) * c > kRescaleThreshold;
+        const float rise = (mx - m) * c;
+        const bool need = !fresh && (kDiff ? !(rise <= kRescaleThreshold) : rise > kRescaleThreshold);  // differential: NaN is taken over and kept
         const float alpha = need ? ex2f((m - mx) * c) : 1.f;
-        m = (fresh || need) ? mx : m;
+        m = (fresh || need) ? (kDiff ? fmax_nan(m, mx) : mx) : m;
         if (__any_sync(0xffffffffu, need)) {
           // S(j) complete implies that the PV MMAs of block j-1 have finished accumulating into O
           l *= alpha;
@@ -687,7 +690,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 x = ffma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, nm2);
-            const float2 e = kDiff && i % kPolynomialEvery == kPolynomialEvery - 1 ? exp2_polynomial(x) : make_float2(ex2f(x.x), ex2f(x.y));
+            const float2 e = kDiff && i % kPolynomialEvery == kPolynomialEvery - 1 ? exp2_polynomial<false>(x) : make_float2(ex2f(x.x), ex2f(x.y));
             sum[i & 3] = fadd2(sum[i & 3], e);  // independent chains, as for the maximum
             pk[i] = pack_half2(e.x, e.y);
           }
@@ -726,8 +729,10 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
       __half* orow = p.o + o_index;
       if constexpr (kDiff) {
         // this warp's factor to the other map's warp of the same rows, and half of the columns of both maps' rows
+        // A row that a NaN or an infinite score reaches keeps NaN in the factor and the LSE.
         float inv = 0.f, lse_val = 0.f;
-        if (nbt > 0 && l > 0.f && m != -INFINITY) {
+        if (nbt > 0 && m != -INFINITY) {
+          l += m - m;  // an infinite maximum: NaN
           inv = 1.f / l;
           lse_val = (m * c + __log2f(l)) * kLn2;
         }

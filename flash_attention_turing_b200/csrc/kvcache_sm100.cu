@@ -454,7 +454,7 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
           sc[w] = (mw[w] == -INFINITY) ? 0.f : ex2f((mw[w] - mt) * c);
           lt += lw[w] * sc[w];
         }
-        const bool dead = (mt == -INFINITY) || (lt == 0.f);
+        const bool dead = (mt == -INFINITY && lt == lt) || lt == 0.f;  // a row of NaN scores has no maximum either, but a sum of NaN
         const float inv = dead ? 0.f : 1.f / lt;
         float acc[kColsPerThread];
 #pragma unroll
@@ -671,9 +671,9 @@ __device__ __forceinline__ float merge_row(const float* o_accum, const float* ls
   fetch(0);
   const float first = lse_of(lane);
   float mx = first;
-  for (int j = lane + 32; j < parts; j += 32) mx = fmaxf(mx, lse_of(j));
+  for (int j = lane + 32; j < parts; j += 32) mx = fmax_nan(mx, lse_of(j));
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  for (int off = 16; off > 0; off >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   const bool dead = mx == -INFINITY;
   float sum = 0.f, weight = 0.f;
 #pragma unroll
@@ -894,7 +894,7 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
             for (int e = 0; e < kPerLane; ++e) acc[e] = fmaf(x[e], scale, acc[e]);
           }
-          const bool dead = mt == -INFINITY || lt == 0.f;
+          const bool dead = (mt == -INFINITY && lt == lt) || lt == 0.f;  // as in the split kernel
           if (dead) {  // no visible key: 0 times a value that is hidden may be NaN
 #pragma unroll
             for (int e = 0; e < kPerLane; ++e) acc[e] = 0.f;

@@ -525,10 +525,24 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// NaN where one of them is: the merges of partial rows must not drop a part whose LSE is NaN
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // 2^x without the special-function unit, for x up to 127: x = n + f with n the nearest integer, a polynomial of degree 4 in f (its
 // coefficients minimise the largest relative error over [-1/2, 1/2], 2.7e-6), and n added to the exponent.  Below -125 (masked scores
-// are -inf): 2^-125, far below what fp16 and the row sums hold.  NaN stays NaN or becomes infinite.
+// are -inf): 2^-125, far below what fp16 and the row sums hold.  The usual NaN then comes out as the
+// largest finite number; with kKeepsNan 2^n is a factor, and it stays NaN.  (In the forward kernel that took 1.03 of the time at D = 64 without
+// mask; there the row maximum carries the NaN to the exponentials beside this one.)
+template <bool kKeepsNan>
 __device__ __forceinline__ float2 exp2_polynomial(float2 x) {
   asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x.x));  // -125
   asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x.y));
@@ -538,8 +552,9 @@ __device__ __forceinline__ float2 exp2_polynomial(float2 x) {
   p = ffma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
   p = ffma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
   p = ffma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  const int nx = __float_as_int(t.x) << 23, ny = __float_as_int(t.y) << 23;
+  if constexpr (kKeepsNan) return fmul2(p, make_float2(__int_as_float(nx + 0x3f800000), __int_as_float(ny + 0x3f800000)));
+  return make_float2(__int_as_float(__float_as_int(p.x) + nx), __int_as_float(__float_as_int(p.y) + ny));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
