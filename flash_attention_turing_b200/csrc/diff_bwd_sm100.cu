@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
   const int sub = threadIdx.x % tpr;
   const int head = item % p.h, row0 = (item / p.h) * kPreRows, batch = blockIdx.z;
   const int q_off = p.cu_seqlens_q ? p.cu_seqlens_q[batch] : 0;
-  const int sq = min(p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - q_off : p.seqlen_q, p.sq_pad);
+  const int sq = p.cu_seqlens_q ? min(p.cu_seqlens_q[batch + 1] - q_off, p.seqlen_q) : p.seqlen_q;  // rows past max_seqlen_q have no LSE
   auto base = [&](int64_t batch_stride, int64_t row_stride, int64_t head_stride) {
     return (p.cu_seqlens_q ? q_off * row_stride : batch * batch_stride) + head * head_stride + sub * 8;
   };
@@ -182,14 +182,16 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
 #pragma unroll 1
       for (int i = 0; i < 3; ++i) clear_unused_rows(p.clear[i], stopped, worker, static_cast<uint32_t>(blocks) * kClearThreads);
     }
-    // keys past max_seqlen_k: the first blocks of the sequence
-    const int* cu_k = p.clear[1].cu_seqlens;
-    const int64_t first = static_cast<int64_t>(cu_k[batch]) + p.keys_written;
-    const int64_t last = min(static_cast<int64_t>(cu_k[batch + 1]), p.clear[1].total);
+    // rows past max_seqlen_q and keys past max_seqlen_k: the first blocks of the sequence
     const uint32_t workers = min(gridDim.x, static_cast<unsigned>(kMaxClearBlocks)) * kClearThreads;
-    if (first < last && blockIdx.x < kMaxClearBlocks) {
+    if (blockIdx.x < kMaxClearBlocks) {
 #pragma unroll 1
-      for (int i = 1; i < 3; ++i) clear_rows(p.clear[i], first, last, blockIdx.x * kClearThreads + threadIdx.x, workers);
+      for (int i = 0; i < 3; ++i) {
+        const int* cu = p.clear[i].cu_seqlens;
+        const int64_t first = static_cast<int64_t>(cu[batch]) + (i == 0 ? p.seqlen_q : p.keys_written);
+        const int64_t last = min(static_cast<int64_t>(cu[batch + 1]), p.clear[i].total);
+        clear_rows(p.clear[i], first, last, blockIdx.x * kClearThreads + threadIdx.x, workers);
+      }
     }
   }
 }
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(256, 3) diff_preprocess_kernel(const __grid_co
 __device__ __forceinline__ void sum_dlam(const DiffKernelParams& p, int head, int lane) {
   constexpr int kLoads = 8;
   auto rows_of = [&](int batch) {
-    return min(p.cu_seqlens_q ? p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch] : p.seqlen_q, p.sq_pad);
+    return p.cu_seqlens_q ? min(p.cu_seqlens_q[batch + 1] - p.cu_seqlens_q[batch], p.seqlen_q) : p.seqlen_q;
   };
   auto stats_of = [&](int batch) {
     return p.stats + (static_cast<int64_t>(batch) * p.h + head) * (p.sq_pad / kStatRows) * kStatFloats + 3 * kStatRows;

@@ -897,7 +897,7 @@ fwd_kernel(const __grid_constant__ FwdKernelParams p) {
   }
 }
 
-// FA_FWD_ZERO_UNUSED_ROWS: the rows of O outside every sequence, and those of the LSE past the end of each.  The forward kernel, which
+// FA_FWD_ZERO_UNUSED_ROWS: the rows of O outside every sequence and past rows_written of each, and those of the LSE past the end of each.  The forward kernel, which
 // writes all other rows, is launched and sets itself up under this one, and waits for it before its first load.  (The LSE was cleared
 // whole by a launch of its own: 4 us of the host and 2 of the GPU per call.)
 struct UnusedLse {
@@ -907,10 +907,16 @@ struct UnusedLse {
 };
 constexpr int kLseChunk = 4 * kClearThreads;
 __global__ void __launch_bounds__(kClearThreads) clear_unused_rows_kernel(const __grid_constant__ PackedRows t,
-                                                                           const __grid_constant__ UnusedLse l, const int* status) {
+                                                                           const __grid_constant__ UnusedLse l, int rows_written,
+                                                                           const int* status) {
   grid_launch_dependents();
   const bool stopped = wait_timed_out(status);
   clear_unused_rows(t, stopped, blockIdx.x * kClearThreads + threadIdx.x, gridDim.x * kClearThreads);
+  if (rows_written < t.total) {
+    for (int batch = blockIdx.x; batch < t.b; batch += gridDim.x)
+      clear_rows(t, static_cast<int64_t>(t.cu_seqlens[batch]) + rows_written, min(static_cast<int64_t>(t.cu_seqlens[batch + 1]), t.total),
+                 threadIdx.x, kClearThreads);
+  }
   const int chunks = (l.seqlen_q + kLseChunk - 1) / kLseChunk;
   for (int64_t u = blockIdx.x; u < static_cast<int64_t>(l.b) * l.h * chunks; u += gridDim.x) {
     const int64_t bh = u / chunks;
@@ -1071,7 +1077,8 @@ int run_fwd(const FaFwdParams* p, int seqused_k_add, cudaStream_t stream, bool o
     const int sms = device_sm_count();
     if (sms <= 0) return set_error(FA_ERR_CUDA, "fa_fwd: device attributes not available");
     const UnusedLse lse{p->lse, p->lse_row_stride, lse_batch, p->h, p->seqlen_q};
-    clear_unused_rows_kernel<<<sms, kClearThreads, 0, stream>>>(rows, lse, kp.status);
+    const int rows_written = diff ? p->seqlen_q : 0x7fffffff;
+    clear_unused_rows_kernel<<<sms, kClearThreads, 0, stream>>>(rows, lse, rows_written, kp.status);
     FA_CHECK_CUDA(cudaGetLastError());
     overlap = true;
     kp.behind_clear = 1;

@@ -77,7 +77,8 @@ def flash_diff_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
                                 cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
                                 softmax_scale: Optional[float] = None, causal: bool = False) -> torch.Tensor:
     """Packed sequences: q (total_q, nheads, d); k, v (total_k, nheads_k, d); cu_seqlens_* int32 (batch + 1,) -> out like q.
-    Rows outside every sequence are zero in the output and in the gradients and count for nothing."""
+    Rows outside every sequence are zero in the output and in the gradients and count for nothing, and so are those of a sequence past
+    max_seqlen_q."""
     out = _gpu().diff_attention_varlen(q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal)
     if out is not None:
         return out

@@ -357,8 +357,8 @@ int fa_sum_gather(const FaSumGatherParams* p, fa_stream_t stream);
 /* above (`base`), with these differences: q and k are cut in two along d (softmax_scale is applied */
 /* as given, (d / 2)^-1/2 is usual, at least 1e-6); base.lse holds two rows per head, (b, 2 * h, lse_row_stride),   */
 /* row 2 * head + map; a row without a visible key gets O = 0 and both LSE = 0; FA_FWD_ZERO_UNUSED_ROWS */
-/* clears rows of O, not of the LSE.  No counterpart in                                           */
-/* the reference.                                                                                 */
+/* clears rows of O, not of the LSE; rows of a packed sequence past seqlen_q (which has to be the longest) are not computed, */
+/* count for nothing in the gradients, and are among those that the two flags clear.  No counterpart in the reference.  */
 /* ------------------------------------------------------------------------------------------- */
 typedef struct FaDiffWeights {
   const void* lam;    /* fp32 or fp16                                                            */

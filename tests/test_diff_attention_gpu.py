@@ -512,3 +512,32 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="lam must be"):
         fa.flash_diff_attn_with_kvcache(q, k, k, lam.double(), cache_seqlens=2)
     assert fa.device_status() == 0
+
+
+@pytest.mark.parametrize("lens,longest,d,causal", [([150, 40], 100, 64, True), ([70, 400, 3], 130, 128, False), ([129], 128, 128, True), ([300, 300], 1, 64, False)])
+def test_sequences_longer_than_the_given_maximum(lens, longest, d, causal):
+    """Rows past max_seqlen_q have no place in the LSE: they are zero and count for nothing, whatever the memory held before."""
+    gen = _gen(17)
+    n, h, hk = sum(lens), 4, 2
+    cu = torch.tensor([0] + lens).cumsum(0).int().cuda()
+    leaves = [t.requires_grad_() for t in (_randn(gen, n, h, d), _randn(gen, n, hk, d), _randn(gen, n, hk, d), _lam(gen, h))]
+    dout = _randn(gen, n, h, d)
+    torch.cuda.empty_cache()
+    memory = torch.full((32 << 20,), 255, dtype=torch.uint8, device="cuda")
+    del memory
+    out = fa.flash_diff_attn_varlen_func(*leaves, cu, cu, longest, max(lens), causal=causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    dlam, bound = 0, 0
+    for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+        s, past = slice(a, b), slice(min(a + longest, b), b)
+        counted = dout[s].clone()
+        counted[longest:] = 0
+        want = sequence(leaves[0][s], leaves[1][s], leaves[2][s], leaves[3], causal, counted)
+        check(out[a:past.start], tuple(t[:longest] for t in want["out"]), "out")
+        assert not out[past].any() and not grads[0][past].any()
+        check(grads[0][a:past.start], tuple(t[:longest] for t in want["dq"]), "dq")
+        check(grads[1][s], want["dk"], "dk")
+        check(grads[2][s], want["dv"], "dv")
+        dlam, bound = dlam + want["dlam"][0], bound + want["dlam"][1]
+    check_dlam(grads[3], (dlam, bound))
+    assert fa.device_status() == 0
