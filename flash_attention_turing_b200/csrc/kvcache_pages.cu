@@ -152,7 +152,8 @@ struct ForkParams {
 };
 constexpr int kRefused = 0x7fffffff;
 
-// Whether a parent's pages can be shared, apart from what its child is; partial: the last one has to be copied
+// Whether a parent's pages can be shared, apart from what its child is and from a hole among them (see fork_row); partial: the last one
+// has to be copied
 __device__ __forceinline__ bool forkable(const FaPageTables& t, int parent, int page_size, bool& partial) {
   const int64_t len = max(t.cache_seqlens[parent], 0), pages = pages_of(len, page_size);
   const int held = held_pages(t, parent, pages);
@@ -160,12 +161,17 @@ __device__ __forceinline__ bool forkable(const FaPageTables& t, int parent, int 
   return held > 0 && held >= pages && (!partial || t.block_table[parent * t.row_stride + pages - 1] < t.num_pages);
 }
 
-// The tables of a child, by a warp; page: for the parent's last tokens, -1: its pages are full
-__device__ __forceinline__ void fork_row(const FaPageTables& t, int parent, int child, int page_size, int page) {
+// The tables of a child, by a warp; page: for the parent's last tokens, -1: its pages are full.  Whether it was done: not for a parent
+// with -1 before its last page.  No function leaves such a row; it is found here, where all entries are read, and the page that was meant
+// for the copy stays free.
+__device__ __forceinline__ bool fork_row(const FaPageTables& t, int parent, int child, int page_size, int page) {
   const int lane = threadIdx.x & 31;
   const int len = max(t.cache_seqlens[parent], 0), full = len / page_size;
   const int* from = t.block_table + parent * t.row_stride;
   int* to = t.block_table + child * t.row_stride;
+  bool whole = true;
+  for (int c = lane; c < full; c += 32) whole &= from[c] >= 0;
+  if (!__all_sync(0xffffffffu, whole)) return false;
   for (int c = lane; c < full; c += 32) {
     const int shared = from[c];
     to[c] = shared;
@@ -178,6 +184,7 @@ __device__ __forceinline__ void fork_row(const FaPageTables& t, int parent, int 
     }
     t.cache_seqlens[child] = len;
   }
+  return true;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constant__ ForkParams p) {
@@ -208,15 +215,17 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constan
   __syncthreads();  // the ranks
   for (int i = threadIdx.x >> 5; i < p.n; i += kPlanWarps) {  // a warp per entry
     const int rank = p.begin[i];
-    const bool granted = rank < found;  // kRefused is not, an entry that needs no page is
-    if ((threadIdx.x & 31) == 0) p.granted[i] = granted;
-    if (!granted) continue;
+    if (rank >= found) {  // kRefused is, an entry that needs no page is not
+      if ((threadIdx.x & 31) == 0) p.granted[i] = false;
+      continue;
+    }
     const int parent = p.parents[i], page = rank >= 0 ? p.list[rank] : -1;
     if ((threadIdx.x & 31) == 0 && rank >= 0) {
       const int len = max(p.t.cache_seqlens[parent], 0), full = len / p.page_size;
       p.moves[rank] = PageMove{p.t.block_table[parent * p.t.row_stride + full], page, (len - full * p.page_size) * p.token_bytes};
     }
-    fork_row(p.t, parent, p.children[i], p.page_size, page);
+    const bool done = fork_row(p.t, parent, p.children[i], p.page_size, page);
+    if ((threadIdx.x & 31) == 0) p.granted[i] = done;
   }
 }
 
@@ -509,9 +518,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_few_kernel(const __grid_con
   if (tid == 0) *p.counter = 0;
   for (int i = warp; i < p.n; i += kWarps) {
     int page;
-    const bool done = plan(i, page);
+    const bool done = plan(i, page) && fork_row(p.t, parents[i], children[i], p.page_size, page);
     if (lane == 0) p.granted[i] = done;
-    if (done) fork_row(p.t, parents[i], children[i], p.page_size, page);
   }
 }
 

@@ -416,3 +416,30 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=text):
             call()
     c.compare()
+
+
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_a_parent_whose_row_has_a_hole_is_not_forked(n):
+    """-1 before the last page, which no function leaves: refused, and nothing is counted in front of page_refs."""
+    rows, pages, page = n + 3, 120, 16
+    memory = torch.zeros(pages + 64, dtype=torch.int32, device="cuda")
+    refs = memory[32:32 + pages]
+    table = torch.full((rows, 4), -1, dtype=torch.int32, device="cuda")
+    table[0], table[1], table[2] = _int([3, -1, 5, -1]), _int([0, 1, 2, -1]), _int([6, -1, 7, 8])
+    for p in (3, 5, 0, 1, 2, 6, 7, 8):
+        refs[p] = 1
+    lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    lens[:3] = _int([3 * page, 2 * page + 5, 3 * page + 2])  # full pages; a last one to copy; and one behind a hole
+    cache = torch.arange(pages, device="cuda").half()[:, None, None].expand(pages, page, 64).contiguous()
+    before = table.clone()
+    parents = [(0, 2, 1)[i % 3] for i in range(n)]
+    got = fa.kvcache_fork([cache], table, lens, refs, _int(parents), _int(list(range(3, rows)))).tolist()
+    assert got == [p == 1 for p in parents]
+    assert not memory[:32].any() and not memory[32 + pages:].any() and torch.equal(table[:3], before[:3])
+    copies = sum(got)
+    assert refs[:3].tolist() == [1 + copies, 1 + copies, 1] and refs.sum().item() == 8 + 3 * copies
+    for i, (p, ok) in enumerate(zip(parents, got)):
+        row, length = table[3 + i].tolist(), lens[3 + i].item()
+        assert (row[:2] == [0, 1] and row[3] == -1 and length == 2 * page + 5) if ok else (row == [-1] * 4 and length == 0)
+        if ok:
+            assert (cache[row[2], :5] == 2).all() and refs[row[2]] == 1
