@@ -431,7 +431,7 @@ struct FewForkParams {
   uint8_t* granted;
   int64_t token_bytes;
   int* counter;  // zero before and after
-  int caches, chunks, ctas, n, page_size;  // ctas: for the chunks of a page of a cache
+  int caches, ctas, n, page_size;  // ctas: for the chunks of a page of a cache
 };
 template <int kUnroll>
 __global__ void __launch_bounds__(kCopyThreads) fork_few_kernel(const __grid_constant__ FewForkParams p) {
@@ -608,16 +608,15 @@ int launch_moves(const FaPageCaches* c, const PageMove* moves, const int* count,
 }
 
 // CTAs for each cache of an entry: all of them are resident together, and they read 32 MB of counts between them at most
-int few_fork_ctas(const FaPageCaches* c, int n, int* units, int* chunks) {
+int few_fork_ctas(const FaPageCaches* c, int n, int* units) {
   *units = chunk_units(n * c->count * c->page_bytes, 148);
-  const int64_t chunk = *units * kCopyThreads * 16;
-  *chunks = static_cast<int>((c->page_bytes + chunk - 1) / chunk);
-  return std::min(*chunks, kFewForkCtas / (n * c->count));
+  const int64_t chunk = *units * kCopyThreads * 16, chunks = (c->page_bytes + chunk - 1) / chunk;
+  return static_cast<int>(std::min<int64_t>(chunks, kFewForkCtas / (n * c->count)));
 }
 bool forks_few(const FaPageTables* t, const FaPageCaches* c, int n) {
   if (n < 1 || n > kFewForks || c->count < 1 || c->count > kMaxCaches || c->page_bytes < 16 || c->page_bytes >= (1 << 30)) return false;
-  int units, chunks;
-  const int64_t ctas = few_fork_ctas(c, n, &units, &chunks);
+  int units;
+  const int64_t ctas = few_fork_ctas(c, n, &units);
   return ctas >= 1 && n * c->count * ctas * t->num_pages <= (8 << 20);
 }
 
@@ -630,7 +629,7 @@ int launch_few_forks(const FaPageTables* t, const FaPageCaches* c, const int* pa
   p.counter = next_sched_slot(stream);
   if (p.counter == nullptr) return set_error(FA_ERR_CUDA, "fa_pages_fork: device attributes not available");
   int units;
-  p.ctas = few_fork_ctas(c, n, &units, &p.chunks);
+  p.ctas = few_fork_ctas(c, n, &units);
   const auto kernel = units == 8 ? fork_few_kernel<8> : units == 2 ? fork_few_kernel<2> : fork_few_kernel<1>;
   kernel<<<n * c->count * p.ctas, kCopyThreads, 0, stream>>>(p);
   FA_CHECK_CUDA(cudaGetLastError());
