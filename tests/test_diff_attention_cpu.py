@@ -92,3 +92,15 @@ def test_struct_layouts_match_the_header(tmp_path):
     subprocess.run(["gcc", "-std=c99", "-I", str(HEADER.parent), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(getattr(capi, n)) for n in names]
+
+
+@built
+@pytest.mark.parametrize("b,longest,total,h", [(1000, 8192, 8192 + 999 * 24, 16), (4096, 4096, 200000, 8), (3, 100, 220, 4), (1, 5000, 5000, 32)])
+def test_scratch_memory_of_a_packed_backward_follows_the_tokens(b, longest, total, h):
+    """Whatever the longest sequence: 148 bytes for each head and row of 64-row tiles, of which a sequence fills all but one."""
+    p = capi.FaDiffBwdParams()
+    p.base.b, p.base.seqlen_q, p.base.seqlen_k, p.base.h, p.base.h_k, p.base.d = b, longest, longest, h, h, 64
+    p.base.total_q = p.base.total_k = total
+    p.base.cu_seqlens_q = p.base.cu_seqlens_k = 1 << 20  # never read
+    got = capi.lib().fa_diff_bwd_workspace_bytes(ctypes.byref(p))
+    assert total * h * 148 <= got <= (total + 64 * (b + 1)) * h * 148 + 1024

@@ -541,3 +541,27 @@ def test_sequences_longer_than_the_given_maximum(lens, longest, d, causal):
         dlam, bound = dlam + want["dlam"][0], bound + want["dlam"][1]
     check_dlam(grads[3], (dlam, bound))
     assert fa.device_status() == 0
+
+
+@pytest.mark.parametrize("h,hk,d,causal", [(3, 1, 64, True), (2, 2, 128, False)])
+def test_one_long_sequence_among_many_short_ones(h, hk, d, causal):
+    """Sequences that begin anywhere in the 64-row tiles of the scratch memory, in the middle of a batch and at its ends."""
+    gen = _gen(18)
+    lens = [3, 0, 61, 64, 1] + [i * 5 % 23 for i in range(60)] + [1500] + [(i * 7 + 1) % 90 for i in range(60)] + [128, 0, 65]
+    n = sum(lens)
+    cu = torch.tensor([0] + lens).cumsum(0).int().cuda()
+    leaves = [t.requires_grad_() for t in (_randn(gen, n, h, d), _randn(gen, n, hk, d), _randn(gen, n, hk, d), _lam(gen, h))]
+    dout = _randn(gen, n, h, d)
+    torch.cuda.empty_cache()
+    memory = torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")
+    del memory
+    out = fa.flash_diff_attn_varlen_func(*leaves, cu, cu, 1500, 1500, causal=causal)
+    grads = torch.autograd.grad(out, leaves, dout)
+    dlam, bound = 0, 0
+    for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+        s = slice(a, b)
+        want = sequence(leaves[0][s], leaves[1][s], leaves[2][s], leaves[3], causal, dout[s])
+        for x, name in zip((out, *grads[:3]), ("out", "dq", "dk", "dv")):
+            check(x[s], want[name], name)
+        dlam, bound = dlam + want["dlam"][0], bound + want["dlam"][1]
+    check_dlam(grads[3], (dlam, bound))
