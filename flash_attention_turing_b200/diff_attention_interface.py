@@ -19,7 +19,7 @@ from typing import Optional, Union
 import torch
 
 from . import flash_attention_interface as _interface
-from .flash_attention_interface import _diff_scale, _gpu, _kvcache_step, maybe_contiguous
+from .flash_attention_interface import _diff_scale, _gpu, _kvcache_step, _readable_gradient, maybe_contiguous
 
 
 # The classes answer what the native autograd node leaves to them: functorch transforms, tracing, modes, tensor subclasses,
@@ -39,7 +39,7 @@ class FlashDiffAttnFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, lam, out, o2, lse = ctx.saved_tensors
-        dq, dk, dv, dlam = _gpu().diff_bwd(q, k, v, lam, out, o2, lse, maybe_contiguous(dout), ctx.softmax_scale, ctx.causal)
+        dq, dk, dv, dlam = _gpu().diff_bwd(q, k, v, lam, out, o2, lse, _readable_gradient(dout), ctx.softmax_scale, ctx.causal)
         return dq, dk, dv, dlam, None, None, None
 
 
@@ -60,7 +60,7 @@ class FlashDiffAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, lam, out, o2, lse, cu_q, cu_k = ctx.saved_tensors
-        dq, dk, dv, dlam = _gpu().diff_varlen_bwd(q, k, v, lam, out, o2, lse, maybe_contiguous(dout), cu_q, cu_k, *ctx.lengths,
+        dq, dk, dv, dlam = _gpu().diff_varlen_bwd(q, k, v, lam, out, o2, lse, _readable_gradient(dout), cu_q, cu_k, *ctx.lengths,
                                                   ctx.softmax_scale, ctx.causal)
         return dq, dk, dv, dlam, None, None, None, None, None, None, None
 

@@ -1,0 +1,49 @@
+"""Gradients of outputs in the layouts that autograd makes of what follows the attention: expanded, sliced, not aligned to 16 bytes."""
+import pytest
+import torch
+
+import flash_attention_turing_b200 as fa
+from flash_attention_turing_b200 import diff_attention_interface, flash_attention_interface
+
+pytestmark = pytest.mark.gpu
+
+
+def _layouts(shape, gen):
+    """Gradients of `shape` (rows.., heads, d)."""
+    rand = lambda *s: torch.randn(*s, generator=gen).half().cuda()  # noqa: E731
+    *rows, h, d = shape
+    yield "sum over rows", rand(1, h, d).expand(*rows, h, d) if len(rows) == 1 else rand(rows[0], 1, h, d).expand(shape)
+    yield "sum over everything in front", rand(*[1] * len(rows), h, d).expand(shape)
+    yield "one for all heads", rand(*rows, 1, d).expand(shape)
+    yield "sum over all", rand(1).expand(shape)
+    yield "slice of wider heads", rand(*rows, h, d + 3)[..., 3:]
+    yield "slice at an odd element", rand(*rows, h * d + 1)[..., 1:].unflatten(-1, (h, d))
+    yield "transposed", rand(*rows, d, h).transpose(-1, -2)
+    yield "whole", rand(*shape)
+
+
+@pytest.mark.parametrize("differential", [True, False])
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("by_class", [True, False])
+def test_gradient_layouts(differential, packed, by_class):
+    gen = torch.Generator().manual_seed(1)
+    shape = (90, 4, 64) if packed else (2, 45, 4, 64)
+    leaves = [torch.randn(*shape[:-2], n, 64, generator=gen).half().cuda().requires_grad_() for n in (4, 2, 2)]
+    if differential:
+        leaves.append(torch.rand(4, generator=gen).cuda().requires_grad_())
+    cu = torch.tensor([0, 50, 90], dtype=torch.int32, device="cuda")
+    more = (cu, cu, 50, 50) if packed else ()
+    module = diff_attention_interface if differential else flash_attention_interface
+    if by_class:  # what the native node leaves to it
+        name = "Flash" + ("Diff" if differential else "") + "Attn" + ("Varlen" if packed else "") + "Func"
+        out = getattr(module, name).apply(*leaves, *more, None, True, True)
+    else:
+        name = "flash_" + ("diff_" if differential else "") + "attn_" + ("varlen_" if packed else "") + "func"
+        out = getattr(fa, name)(*leaves, *more, causal=True)
+    out = out[0] if isinstance(out, tuple) else out
+    for name, dout in _layouts(shape, gen):
+        want = torch.autograd.grad(out, leaves, dout.clone(memory_format=torch.contiguous_format), retain_graph=True)
+        got = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+    pooled = out.sum(0 if packed else 1)
+    assert torch.isfinite(torch.autograd.grad((pooled * torch.arange(4, device="cuda")[:, None]).sum(), leaves)[0]).all()
