@@ -25,6 +25,9 @@ void check_supported_head_dim(int64_t d) {
   TORCH_CHECK(d == 64 || d == 128, "Turing FlashAttention supports head_dim 64 or 128");
 }
 
+// a remainder of a division by zero would end the process
+bool heads_divide(int64_t heads, int64_t heads_k) { return heads_k > 0 && heads % heads_k == 0; }
+
 void check_half_cuda(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be a float16 tensor");
@@ -120,7 +123,7 @@ std::vector<at::Tensor> dense_forward(at::Tensor q, at::Tensor k, at::Tensor v, 
   TORCH_CHECK(v.size(1) == seqlen_k, "k and v seqlen_k must match");
   TORCH_CHECK(v.size(2) == num_heads_k, "k and v num_heads must match");
   TORCH_CHECK(k.size(3) == head_size && v.size(3) == head_size, "q/k/v head_dim must match");
-  TORCH_CHECK(num_heads % num_heads_k == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
+  TORCH_CHECK(heads_divide(num_heads, num_heads_k), "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(head_size);
   const int64_t lse_heads = diff ? 2 * num_heads : num_heads;
   if (diff) {
@@ -195,7 +198,7 @@ void check_varlen_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor
   TORCH_CHECK(k.size(1) == v.size(1), "k and v num_heads must match");
   TORCH_CHECK(k.size(2) == v.size(2), "k and v head_dim must match");
   TORCH_CHECK(q.size(2) == k.size(2), "q/k/v head_dim must match");
-  TORCH_CHECK(q.size(1) % k.size(1) == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
+  TORCH_CHECK(heads_divide(q.size(1), k.size(1)), "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(q.size(2));
 }
 
@@ -281,7 +284,7 @@ std::vector<at::Tensor> dense_backward(at::Tensor q, at::Tensor k, at::Tensor v,
   TORCH_CHECK(v.size(2) == num_heads_k, "k and v num_heads must match");
   TORCH_CHECK(k.size(3) == head_size && v.size(3) == head_size, "q/k/v head_dim must match");
   TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(), "out and dout must match q shape");
-  TORCH_CHECK(num_heads % num_heads_k == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
+  TORCH_CHECK(heads_divide(num_heads, num_heads_k), "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(head_size);
   check_lse_view(l, batch_size, diff ? 2 * num_heads : num_heads, seqlen_q, "l");
   if (diff) {
@@ -731,7 +734,7 @@ std::vector<at::Tensor> kvcache_forward(Verdict* checked, at::Tensor q, at::Tens
   TORCH_CHECK(k_cache.size(2) == v_cache.size(2), "k_cache and v_cache num_heads must match");
   TORCH_CHECK(q.size(3) == k_cache.size(3) && q.size(3) == v_cache.size(3),
               "q, k_cache, v_cache head_dim must match");
-  TORCH_CHECK(q.size(2) % k_cache.size(2) == 0, "num_heads_q must be divisible by num_heads_k for GQA/MQA");
+  TORCH_CHECK(heads_divide(q.size(2), k_cache.size(2)), "num_heads_q must be divisible by num_heads_k for GQA/MQA");
   check_supported_head_dim(q.size(3));
   TORCH_CHECK(q.stride(-1) == 1 && k_cache.stride(-1) == 1 && v_cache.stride(-1) == 1,
               "q, k_cache, v_cache must have contiguous last dimension");

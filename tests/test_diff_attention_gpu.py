@@ -565,3 +565,17 @@ def test_one_long_sequence_among_many_short_ones(h, hk, d, causal):
             check(x[s], want[name], name)
         dlam, bound = dlam + want["dlam"][0], bound + want["dlam"][1]
     check_dlam(grads[3], (dlam, bound))
+
+
+def test_no_key_heads():
+    """Refused by every entry point, plain and differential: the number of query heads is not divided by zero."""
+    q, k, lam = torch.zeros(1, 4, 4, 64, device="cuda").half(), torch.zeros(1, 4, 0, 64, device="cuda").half(), torch.zeros(4, device="cuda")
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    for more in ((), (lam,)):
+        names = ("flash_diff_attn_func", "flash_diff_attn_varlen_func", "flash_diff_attn_with_kvcache") if more else (
+            "flash_attn_func", "flash_attn_varlen_func", "flash_attn_with_kvcache")
+        dense, packed, cached = (getattr(fa, n) for n in names)
+        for call in (lambda: dense(q, k, k, *more), lambda: packed(q[0], k[0], k[0], *more, cu, cu, 4, 4),
+                     lambda: cached(q, k, k, *more, cache_seqlens=2), lambda: cached(q, k, k, *more, k, k, cache_seqlens=0)):
+            with pytest.raises((RuntimeError, ValueError)):
+                call()
