@@ -806,6 +806,7 @@ std::vector<at::Tensor> kvcache_forward(Verdict* checked, at::Tensor q, at::Tens
     check_same_device(q, {k_cache, v_cache, cache_seqlens});
     if (has_k) check_same_device(q, {k, v});
     if (has_block_table) check_same_device(q, {block_table});
+    if (has_cache_batch_idx) check_same_device(q, {cache_batch_idx});
     TORCH_CHECK(v_cache.size(0) == k_cache.size(0), "k_cache and v_cache must have the same number of rows or pages");
     diff_weights(*lam, q, num_heads);
   }

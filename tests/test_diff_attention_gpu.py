@@ -579,3 +579,11 @@ def test_no_key_heads():
                      lambda: cached(q, k, k, *more, cache_seqlens=2), lambda: cached(q, k, k, *more, k, k, cache_seqlens=0)):
             with pytest.raises((RuntimeError, ValueError)):
                 call()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="a tensor on another device")
+def test_a_cache_index_on_another_device_is_refused():
+    q, k, lam = torch.zeros(1, 1, 4, 64, device="cuda:0").half(), torch.zeros(1, 64, 2, 64, device="cuda:0").half(), torch.zeros(4, device="cuda:0")
+    idx = torch.zeros(1, dtype=torch.int32, device="cuda:1")
+    with pytest.raises(RuntimeError, match="device of q"):
+        fa.flash_diff_attn_with_kvcache(q, k, k, lam, cache_seqlens=2, cache_batch_idx=idx)
