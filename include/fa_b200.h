@@ -378,7 +378,7 @@ int fa_diff_fwd(const FaDiffFwdParams* p, fa_stream_t stream);
 
 /* Backward: dq, dk, dv (per KV head, summed over its query heads) and the gradient of the weights. */
 /* base.flags: 0 or FA_BWD_ZERO_UNUSED_ROWS; base.workspace holds fa_diff_bwd_workspace_bytes().   */
-/* Every gradient is bitwise reproducible.  dk and dv must not lie over k and v.                   */
+/* Every gradient is bitwise reproducible.  The kernels overlap: dq, dk and dv must not lie over q, k, v or dout. */
 typedef struct FaDiffBwdParams {
   FaBwdParams base;   /* o, lse: what fa_diff_fwd() wrote                                        */
   FaDiffWeights weights;
