@@ -485,8 +485,8 @@ at::Tensor last_dim_contiguous(const at::Tensor& t) {
   return t.numel() == 0 ? torch::empty(t.sizes(), t.options()) : t.contiguous();
 }
 
-// The gradient of an output, in the layout that autograd gives it: see _readable_gradient in flash_attention_interface.py
-at::Tensor readable_gradient(const at::Tensor& t) {
+// See _readable in flash_attention_interface.py
+at::Tensor readable(const at::Tensor& t) {
   bool whole = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) whole = whole && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
   return whole ? t : t.numel() == 0 ? torch::empty(t.sizes(), t.options()) : t.clone(at::MemoryFormat::Contiguous);
@@ -516,7 +516,7 @@ Qkv unpack(const Call& c, const at::Tensor& a, const at::Tensor& b, const at::Te
 
 // diff: differential attention, and what it has besides q, k and v
 std::vector<at::Tensor> attend(const Call& c, const Qkv& x, const at::Tensor& cu_q, const at::Tensor& cu_k, Differential* diff) {
-  const at::Tensor q = last_dim_contiguous(x.q), k = last_dim_contiguous(x.k), v = last_dim_contiguous(x.v);
+  const at::Tensor q = readable(x.q), k = readable(x.k), v = readable(x.v);
   if (c.varlen) return varlen_forward(q, k, v, cu_q, cu_k, c.max_q, c.max_k, c.scale, c.causal, diff);
   return dense_forward(q, k, v, c.scale, c.causal, c10::nullopt, c10::nullopt, c10::nullopt, diff);
 }
@@ -568,8 +568,8 @@ struct Attention : public torch::autograd::Function<Attention> {
     Differential diff;
     if (saved.size() > extra) diff = Differential{saved[extra], true, saved[extra + 1], {}};
     Differential* which = saved.size() > extra ? &diff : nullptr;
-    const at::Tensor dout = readable_gradient(grads[0]), out = last_dim_contiguous(saved[3]), lse = last_dim_contiguous(saved[4]);
-    const at::Tensor cq = last_dim_contiguous(q), ck = last_dim_contiguous(k), cv = last_dim_contiguous(v);
+    const at::Tensor dout = readable(grads[0]), out = last_dim_contiguous(saved[3]), lse = last_dim_contiguous(saved[4]);
+    const at::Tensor cq = readable(q), ck = readable(k), cv = readable(v);
     auto g = c.varlen ? varlen_backward(cq, ck, cv, out, lse, dout, saved[5], saved[6], c.max_q, c.max_k, c.scale, c.causal, dq, dk, dv, which)
                       : dense_backward(cq, ck, cv, out, lse, dout, c.scale, c.causal, dq, dk, dv, c10::nullopt, which);
     const at::Tensor none;  // one entry per argument of forward()

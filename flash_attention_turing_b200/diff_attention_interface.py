@@ -19,7 +19,7 @@ from typing import Optional, Union
 import torch
 
 from . import flash_attention_interface as _interface
-from .flash_attention_interface import _diff_scale, _gpu, _kvcache_step, _readable_gradient, maybe_contiguous
+from .flash_attention_interface import _diff_scale, _gpu, _kvcache_step, _readable
 
 
 # The classes answer what the native autograd node leaves to them: functorch transforms, tracing, modes, tensor subclasses,
@@ -28,7 +28,7 @@ class FlashDiffAttnFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, softmax_scale, causal, is_grad_enabled):
         scale = _diff_scale(q, softmax_scale)
-        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        q, k, v = (_readable(t) for t in (q, k, v))
         keep = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
         out, lse, *o2 = _gpu().diff_fwd(q, k, v, lam, scale, causal, keep)
         if keep:
@@ -39,7 +39,7 @@ class FlashDiffAttnFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, lam, out, o2, lse = ctx.saved_tensors
-        dq, dk, dv, dlam = _gpu().diff_bwd(q, k, v, lam, out, o2, lse, _readable_gradient(dout), ctx.softmax_scale, ctx.causal)
+        dq, dk, dv, dlam = _gpu().diff_bwd(q, k, v, lam, out, o2, lse, _readable(dout), ctx.softmax_scale, ctx.causal)
         return dq, dk, dv, dlam, None, None, None
 
 
@@ -48,7 +48,7 @@ class FlashDiffAttnVarlenFunc(torch.autograd.Function):
     def forward(ctx, q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal,
                 is_grad_enabled):
         scale = _diff_scale(q, softmax_scale)
-        q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+        q, k, v = (_readable(t) for t in (q, k, v))
         keep = is_grad_enabled and any(t.requires_grad for t in (q, k, v, lam))
         out, lse, *o2 = _gpu().diff_varlen_fwd(q, k, v, lam, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, keep)
         if keep:
@@ -60,7 +60,7 @@ class FlashDiffAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, lam, out, o2, lse, cu_q, cu_k = ctx.saved_tensors
-        dq, dk, dv, dlam = _gpu().diff_varlen_bwd(q, k, v, lam, out, o2, lse, _readable_gradient(dout), cu_q, cu_k, *ctx.lengths,
+        dq, dk, dv, dlam = _gpu().diff_varlen_bwd(q, k, v, lam, out, o2, lse, _readable(dout), cu_q, cu_k, *ctx.lengths,
                                                   ctx.softmax_scale, ctx.causal)
         return dq, dk, dv, dlam, None, None, None, None, None, None, None
 

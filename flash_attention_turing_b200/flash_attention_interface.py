@@ -43,11 +43,12 @@ def maybe_contiguous(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return x
 
 
-def _readable_gradient(dout: torch.Tensor) -> torch.Tensor:
-    """The gradient of an output has the layout that autograd gives it: one of a sum over rows is expanded, one of a concatenation a slice.
-    Copied where the kernels, which load 16-byte units through tensor maps, cannot read it as it is."""
-    whole = all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(dout.shape[:-1], dout.stride()[:-1]))
-    return dout if dout.stride(-1) == 1 and whole and dout.data_ptr() % 16 == 0 else dout.contiguous()
+def _readable(x: torch.Tensor) -> torch.Tensor:
+    """Copied where the kernels, which load 16-byte units through tensor maps, cannot read it as it is: expanded, or with rows or
+    heads that are not 16 bytes apart.  The gradient of an output has the layout that autograd gives it (one of a sum over rows is
+    expanded, one of a concatenation a slice), and keys may be broadcast over batch or heads."""
+    whole = all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+    return x if x.stride(-1) == 1 and whole and x.data_ptr() % 16 == 0 else x.contiguous()
 
 
 def _default_scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
@@ -63,7 +64,7 @@ def _diff_scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:
 # thin wrappers around the five bindings (reference :13-169)
 # --------------------------------------------------------------------------------------------
 def _flash_attn_forward(q, k, v, softmax_scale: float, causal: bool):
-    q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+    q, k, v = (_readable(t) for t in (q, k, v))
     out, lse = _gpu().fwd(q, k, v, softmax_scale, causal)
     return out, lse
 
@@ -71,14 +72,14 @@ def _flash_attn_forward(q, k, v, softmax_scale: float, causal: bool):
 def _flash_attn_backward(dout, q, k, v, out, lse, softmax_scale: float, causal: bool, grads=()):
     """``grads``: optional (dq, dk, dv) destinations, e.g. views into one packed gradient tensor; the kernels
     write through their strides, so the packed variants need no concatenation afterwards."""
-    dout, q, k, v, out, lse = (_readable_gradient(dout), *(maybe_contiguous(t) for t in (q, k, v, out, lse)))
+    dout, q, k, v, out, lse = (*(_readable(t) for t in (dout, q, k, v)), maybe_contiguous(out), maybe_contiguous(lse))
     dq, dk, dv = _gpu().bwd(q, k, v, out, lse, dout, softmax_scale, causal, *grads)
     return dq, dk, dv
 
 
 def _flash_attn_varlen_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int, max_seqlen_k: int,
                                softmax_scale: float, causal: bool):
-    q, k, v = (maybe_contiguous(t) for t in (q, k, v))
+    q, k, v = (_readable(t) for t in (q, k, v))
     out, lse = _gpu().varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                                  softmax_scale, causal)
     return out, lse
@@ -86,7 +87,7 @@ def _flash_attn_varlen_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q
 
 def _flash_attn_varlen_backward(dout, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int,
                                 max_seqlen_k: int, softmax_scale: float, causal: bool, grads=()):
-    dout, q, k, v, out, lse = (_readable_gradient(dout), *(maybe_contiguous(t) for t in (q, k, v, out, lse)))
+    dout, q, k, v, out, lse = (*(_readable(t) for t in (dout, q, k, v)), maybe_contiguous(out), maybe_contiguous(lse))
     dq, dk, dv = _gpu().varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
                                    max_seqlen_k, softmax_scale, causal, *grads)
     return dq, dk, dv

@@ -1,4 +1,4 @@
-"""Gradients of outputs in the layouts that autograd makes of what follows the attention: expanded, sliced, not aligned to 16 bytes."""
+"""Inputs and gradients of outputs in layouts that tensor maps do not take: expanded, sliced, not aligned to 16 bytes."""
 import pytest
 import torch
 
@@ -47,3 +47,28 @@ def test_gradient_layouts(differential, packed, by_class):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
     pooled = out.sum(0 if packed else 1)
     assert torch.isfinite(torch.autograd.grad((pooled * torch.arange(4, device="cuda")[:, None]).sum(), leaves)[0]).all()
+
+
+@pytest.mark.parametrize("differential", [True, False])
+@pytest.mark.parametrize("packed", [True, False])
+def test_input_layouts(differential, packed):
+    """Keys and values that are broadcast over heads or batch, slices at odd places: output and gradients as of copies."""
+    gen = torch.Generator().manual_seed(2)
+    rand = lambda *s: torch.randn(*s, generator=gen).half().cuda()  # noqa: E731
+    rows, cu = ((90,) if packed else (2, 45)), torch.tensor([0, 50, 90], dtype=torch.int32, device="cuda")
+    more = (cu, cu, 50, 50) if packed else ()
+    lam = (torch.rand(4, generator=gen).cuda(),) if differential else ()
+    fn = getattr(fa, "flash_" + ("diff_" if differential else "") + "attn_" + ("varlen_" if packed else "") + "func")
+    dout = rand(*rows, 4, 64)
+    for name, base, view in (
+        ("one key head", (rand(*rows, 4, 64), rand(*rows, 1, 64), rand(*rows, 1, 64)), lambda q, k, v: (q, k.expand(*rows, 4, 64), v.expand(*rows, 4, 64))),
+        ("one for all rows", (rand(*[1] * len(rows), 4, 64), rand(*rows, 2, 64), rand(*rows, 2, 64)), lambda q, k, v: (q.expand(*rows, 4, 64), k, v)),
+        ("odd slices", [rand(*rows, n, 67) for n in (4, 2, 2)], lambda *x: [t[..., 3:] for t in x]),
+        ("odd rows", [rand(*rows, n * 64 + 1) for n in (4, 2, 2)], lambda *x: [t[..., 1:].unflatten(-1, (-1, 64)) for t in x]),
+    ):
+        results = []
+        for copied in (False, True):
+            leaves = [t.clone().requires_grad_() for t in base]
+            out = fn(*((t.contiguous() if copied else t) for t in view(*leaves)), *lam, *more, causal=True)
+            results.append([out, *torch.autograd.grad(out, leaves, dout)])
+        assert all(torch.equal(a, b) for a, b in zip(*results)), name
