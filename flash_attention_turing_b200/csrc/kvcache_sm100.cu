@@ -22,9 +22,9 @@
 // (position, head) rows per KV head go to the tiled tcgen05 forward kernel instead (the reference
 // routes them to its tiled kernel too, flash_api.cpp:668-714).
 //
-// Differential attention (kDiff): a query head is two rows of the M dimension, 2 * head + map, whose other half of d is zero, so
-// that K and V are read once for both maps and everything up to the normalised rows is as for two heads (`h` and `group` count
-// rows, and so do the partials and the LSE).  Where a row is stored, its pair is: the warp that has both subtracts them in 32 bits.
+// Differential attention (kDiff): a query head is two rows of the M dimension, 2 * head + map, each with its half of d.  Every row
+// is multiplied with both halves of a key and takes the scores of its own, so that K and V are read once for both maps and everything up to the
+// normalised rows is as for two heads (`h` and `group` count rows, and so do the partials and the LSE).  Where a row is stored, its pair is: the warp that has both subtracts them in 32 bits.
 #include <algorithm>
 #include <mutex>
 
@@ -139,6 +139,7 @@ struct WarpRows {
   float oacc[D / 8][4];
   float m0, m1;           // reference maxima (raw score units)
   float l0, l1;           // per-thread partial row sums
+  int map;                // differential: of both fragment rows
 
   // first: the row of the KV head that is row 0 here
   template <bool kDiff>
@@ -153,17 +154,13 @@ struct WarpRows {
         const int head = head_k * p.group + (r - q_pos * p.group);
         return p.q + batch * p.q_batch_stride + q_pos * p.q_row_stride + (kDiff ? head >> 1 : head) * p.q_head_stride;
       };
-      // differential: the half of d that a row has (groups are even, so rows g and g + 8 have the same)
-      const int map = (first + g) & 1;
+      // differential: D / 32 slices, of the half of d that a row has (groups are even, so rows g and g + 8 have the same)
+      map = (first + g) & 1;
       const __half* r0p = g < rows ? q_ptr(g) : nullptr;
       const __half* r1p = (g + 8) < rows ? q_ptr(g + 8) : nullptr;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int c = k * 16 + t4 * 2;
-        if (kDiff && k / (D / 32) != map) {
-          qa[k][0] = qa[k][1] = qa[k][2] = qa[k][3] = 0u;
-          continue;
-        }
+      for (int k = 0; k < (kDiff ? D / 32 : D / 16); ++k) {
+        const int c = k * 16 + t4 * 2 + (kDiff ? map * (D / 2) : 0);
         qa[k][0] = r0p ? *reinterpret_cast<const uint32_t*>(r0p + c) : 0u;
         qa[k][1] = r1p ? *reinterpret_cast<const uint32_t*>(r1p + c) : 0u;
         qa[k][2] = r0p ? *reinterpret_cast<const uint32_t*>(r0p + c + 8) : 0u;
@@ -183,19 +180,28 @@ struct WarpRows {
   }
 
   // 16 tokens of a tile, the first of them token tok0 < len; sK, sV: the tiles, v_tile: the V tile's address, c: scale * log2(e)
+  template <bool kDiff>
   __device__ __forceinline__ void tokens(uint32_t sK, uint32_t sV, uint8_t* v_tile, int tok_in_tile, int tok0, int len, float c,
                                          int lane) {
     const int t4 = lane & 3;
     // ---- S = Q K^T for 16 tokens: two n8 tiles ----
     float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // differential: every row with both halves of the keys, of which it takes its own (as zeros in the other half the row
+    // would get NaN from an infinite element there)
+    float second[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       uint32_t b0, b1, b2, b3;
       const int mi = lane >> 3, rr = lane & 7;
       ldmatrix_x4(sK + tile_offset<D>(tok_in_tile + (mi >> 1) * 8 + rr, k * 2 + (mi & 1)), b0, b1,
                   b2, b3);
-      mma_16816(sacc[0], qa[k], b0, b1);
-      mma_16816(sacc[1], qa[k], b2, b3);
+      auto& to = kDiff && k >= D / 32 ? second : sacc;
+      mma_16816(to[0], qa[kDiff ? k % (D / 32) : k], b0, b1);
+      mma_16816(to[1], qa[kDiff ? k % (D / 32) : k], b2, b3);
+    }
+    if (kDiff && map != 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sacc[0][i] = second[0][i], sacc[1][i] = second[1][i];
     }
     // ---- mask the tail / causal limit ----
     if (tok0 + 15 > min(lim0, lim1)) {
@@ -402,7 +408,7 @@ decode_split_kernel(const __grid_constant__ DecodeParams p) {
       const uint32_t sK = smem_u32(smem + s * C::kStageBytes);
       const int tok0 = (tile_begin + i) * kTileTokens + tok_in_tile;  // first token of this warp
       if (tok0 < len)
-        w.tokens(sK, sK + C::kTileBytes, smem + s * C::kStageBytes + C::kTileBytes, tok_in_tile, tok0, len, c, lane);
+        w.template tokens<kDiff>(sK, sK + C::kTileBytes, smem + s * C::kStageBytes + C::kTileBytes, tok_in_tile, tok0, len, c, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->empty[s]);
     }
@@ -825,7 +831,7 @@ decode_balanced_kernel(const __grid_constant__ DecodeParams p) {
         uint8_t* stage = smem + (i % C::kStages) * C::kStageBytes;
         const uint32_t sK = smem_u32(stage);
         const int tok0 = (w.tile + t) * kTileTokens + tok_in_tile;
-        if (tok0 < w.len) mine.tokens(sK, sK + C::kTileBytes, stage + C::kTileBytes, tok_in_tile, tok0, w.len, c, lane);
+        if (tok0 < w.len) mine.template tokens<kDiff>(sK, sK + C::kTileBytes, stage + C::kTileBytes, tok_in_tile, tok0, w.len, c, lane);
         release(i);
       }
       ok = ok && wait_full(i);

@@ -169,3 +169,29 @@ def test_plain_cache_step_with_a_query_that_is_not_a_number(length, splits, h):
     assert torch.isnan(got[1, 0, 1]).all()
     got[1, 0, 1] = clean[1, 0, 1]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("b,new,lengths,h,hk,d,page,splits", STEPS)
+def test_a_score_of_minus_infinity_is_a_weight_of_zero(b, new, lengths, h, hk, d, page, splits):
+    """The map that sees it goes by the other keys, the other map by all: the bits are those of an element whose weight underflows."""
+    gen = torch.Generator().manual_seed(6)
+    capacity = -(-(max(lengths) + new) // (page or 64)) * (page or 64)
+    lam = torch.rand(h, generator=gen).cuda() + 0.1
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    table = torch.arange(b * capacity // page, dtype=torch.int32, device="cuda").view(b, -1) if page else None
+    caches = [_rand(gen, b, capacity, hk, d) for _ in range(2)]
+    x = {"q": _rand(gen, b, new, h, d), "k": _rand(gen, b, new, hk, d), "v": _rand(gen, b, new, hk, d)}
+    long = max(range(b), key=lambda i: lengths[i])
+    n = lengths[long]
+    for at in {0, 6, n // 2, n - 1} if n else ():
+        for column in (1, d - 2):
+            outs = []
+            for value in (-INF, -60000.0):
+                keys = caches[0].clone()
+                keys[long, at, 0, column] = value
+                shaped = [t.view(-1, page, hk, d) if page else t for t in (keys, caches[1])]
+                outs.append(_step(fa.flash_diff_attn_with_kvcache, x, lens, table, splits, shaped, lam))
+                dense = [torch.cat((c[long, :n], x[m][long]))[None] for c, m in zip((keys, caches[1]), ("k", "v"))]
+                outs.append(fa.flash_diff_attn_func(x["q"][long:long + 1], *dense, lam, causal=True))
+            assert torch.isfinite(outs[0]).all() and torch.isfinite(outs[1]).all()
+            assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
