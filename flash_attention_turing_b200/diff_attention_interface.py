@@ -9,7 +9,8 @@ Shapes, masks (bottom-right aligned), grouped heads, packed sequences and the KV
 2 * nheads query heads of d / 2 and values of d passes ``q.view(b, s, nheads, d)``: the two maps of a head lie next to each other.
 ``lam`` holds one weight per query head, or a single one for all, fp32 or fp16, and has a gradient.  What a model puts around the
 operator (how lam is parametrised, a norm of the heads' outputs) is its own.  ``softmax_scale`` must be at least 1e-6; the weights should
-lie well inside fp16's range, the type of the products that they enter.
+lie well inside fp16's range, the type of the products that they enter.  A row that sees no key is zero; a NaN, or an infinite score, makes NaN of every
+row that it reaches.
 No counterpart in Cy-47/flash-attention-turing.
 """
 from __future__ import annotations

@@ -47,7 +47,8 @@ def _blame(caches, **tensors) -> None:
 def kvcache_reserve(block_table: torch.Tensor, cache_seqlens: torch.Tensor, page_refs: torch.Tensor,
                     new_tokens: Union[int, torch.Tensor], page_size: int) -> torch.Tensor:
     """Gives every row the pages that ``cache_seqlens + new_tokens`` tokens need (an int for all rows, or int32 (batch,); negative
-    entries count as 0; 0 for rows that are not in use).  Returns bool (batch,): whether the row has them.  Rows are served in order while the free pages last, each
+    entries count as 0).  An int gives pages to rows that are not in use as well, and a row that holds pages cannot become the child of
+    a fork: 0 in a tensor for those.  Returns bool (batch,): whether the row has them.  Rows are served in order while the free pages last, each
     with all it needs or nothing, and what a refused row needs is kept from the rows behind it.  A row whose columns do not suffice is
     refused and keeps nothing from others.  Calling it again for the same tokens changes nothing."""
     each = isinstance(new_tokens, torch.Tensor)
@@ -67,7 +68,7 @@ def kvcache_fork(caches: Sequence[torch.Tensor], block_table: torch.Tensor, cach
     parent's tokens, and the tokens of a last page that is not full are copied to a free page, in every cache.  Pages that the parent has
     reserved ahead are not shared.  A parent may have several children.  Returns bool (n,): whether it was done.  Not done, and
     nothing changed: a row out of range (-1 pads), a child that holds pages or that an earlier entry names, a parent that holds no page
-    or fewer than its length says, or no page left for the copy (entries are served in order)."""
+    or fewer than its length says or has -1 among them, or no page left for the copy (entries are served in order)."""
     caches = _caches(caches)
     try:
         return _ext.load().pages_fork(caches, block_table, cache_seqlens, page_refs, parents, children)

@@ -428,7 +428,8 @@ typedef struct FaPageCaches {
 
 size_t fa_pages_workspace_bytes(int32_t rows, int32_t num_pages, int32_t entries);
 
-/* Pages for cache_seqlens[r] + new_tokens[r] tokens (new_tokens NULL: new_tokens_all each; negative counts as 0).  Rows are   */
+/* Pages for cache_seqlens[r] + new_tokens[r] tokens (new_tokens NULL: new_tokens_all each, unused rows included, which can   */
+/* then not be forked into; negative counts as 0).  Rows are                                                      */
 /* served in order while the free pages last: a row is granted all it needs, or nothing; what a refused row needs counts       */
 /* against the rows behind it.  A row whose columns do not suffice is refused and counts for nothing.  granted[r]: 1 or 0.     */
 size_t fa_pages_reserve_workspace_bytes(const FaPageTables* t);
