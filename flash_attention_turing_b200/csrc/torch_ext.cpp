@@ -488,7 +488,7 @@ at::Tensor last_dim_contiguous(const at::Tensor& t) {
 // See _readable in flash_attention_interface.py
 at::Tensor readable(const at::Tensor& t) {
   bool whole = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) whole = whole && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) whole = whole && (t.size(i) <= 1 || t.stride(i) > 0) && t.stride(i) % 8 == 0;
   return whole ? t : t.numel() == 0 ? torch::empty(t.sizes(), t.options()) : t.clone(at::MemoryFormat::Contiguous);
 }
 

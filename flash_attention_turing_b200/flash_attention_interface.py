@@ -47,8 +47,9 @@ def _readable(x: torch.Tensor) -> torch.Tensor:
     """Copied where the kernels, which load 16-byte units through tensor maps, cannot read it as it is: expanded, or with rows or
     heads that are not 16 bytes apart.  The gradient of an output has the layout that autograd gives it (one of a sum over rows is
     expanded, one of a concatenation a slice), and keys may be broadcast over batch or heads."""
-    whole = all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1]))
-    return x if x.stride(-1) == 1 and whole and x.data_ptr() % 16 == 0 else x.contiguous()
+    whole = all((n <= 1 or s > 0) and s % 8 == 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+    # not contiguous(), to which the stride of a dimension of one element is nothing
+    return x if x.stride(-1) == 1 and whole and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _default_scale(q: torch.Tensor, softmax_scale: Optional[float]) -> float:

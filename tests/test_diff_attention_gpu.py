@@ -587,3 +587,25 @@ def test_a_cache_index_on_another_device_is_refused():
     idx = torch.zeros(1, dtype=torch.int32, device="cuda:1")
     with pytest.raises(RuntimeError, match="device of q"):
         fa.flash_diff_attn_with_kvcache(q, k, k, lam, cache_seqlens=2, cache_batch_idx=idx)
+
+
+def test_keys_past_the_given_maximum():
+    """They are attended, and have no gradients from the next whole tile on."""
+    gen = _gen(19)
+    lens, h, hk, d = [300, 40], 4, 2, 64
+    cu = torch.tensor([0] + lens).cumsum(0).int().cuda()
+    leaves = [t.requires_grad_() for t in (_randn(gen, 340, h, d), _randn(gen, 340, hk, d), _randn(gen, 340, hk, d), _lam(gen, h))]
+    dout = _randn(gen, 340, h, d)
+    torch.cuda.empty_cache()
+    memory = torch.full((32 << 20,), 255, dtype=torch.uint8, device="cuda")
+    del memory
+    out = fa.flash_diff_attn_varlen_func(*leaves, cu, cu, 300, 100, causal=True)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+        s, n = slice(a, b), min(b - a, 128)
+        want = sequence(leaves[0][s], leaves[1][s], leaves[2][s], leaves[3], True, dout[s])
+        check(out[s], want["out"], "out")
+        check(grads[0][s], want["dq"], "dq")
+        for i, name in ((1, "dk"), (2, "dv")):
+            check(grads[i][a:a + n], tuple(t[:n] for t in want[name]), name)
+            assert not grads[i][a + n:b].any()

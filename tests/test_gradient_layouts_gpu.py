@@ -72,3 +72,20 @@ def test_input_layouts(differential, packed):
             out = fn(*((t.contiguous() if copied else t) for t in view(*leaves)), *lam, *more, causal=True)
             results.append([out, *torch.autograd.grad(out, leaves, dout)])
         assert all(torch.equal(a, b) for a, b in zip(*results)), name
+
+
+@pytest.mark.parametrize("differential", [True, False])
+def test_one_row_with_an_odd_stride(differential):
+    """The stride of a dimension of one element, which no address depends on."""
+    gen = torch.Generator().manual_seed(3)
+    leaves = [torch.randn(1, 1, n, 64, generator=gen).half().cuda().requires_grad_() for n in (4, 2, 2)]
+    if differential:
+        leaves.append(torch.rand(4, generator=gen).cuda().requires_grad_())
+    dout = torch.randn(257, generator=gen).half().cuda().as_strided((1, 1, 4, 64), (257, 257, 64, 1))
+    assert dout.stride() == (257, 257, 64, 1) and dout.is_contiguous()
+    for cls in (None, diff_attention_interface.FlashDiffAttnFunc if differential else flash_attention_interface.FlashAttnFunc):
+        fn = fa.flash_diff_attn_func if differential else fa.flash_attn_func
+        out = cls.apply(*leaves, None, False, True) if cls else fn(*leaves)
+        out = out[0] if isinstance(out, tuple) else out
+        want = torch.autograd.grad(out, leaves, dout.clone(memory_format=torch.contiguous_format), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, dout), want))
